@@ -9,7 +9,14 @@ import os
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "lib", "libfeatgraph_hip.so")
 
-_i32, _i64, _p = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+_i32, _i64, _p, _f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
+
+
+class Tensor(ctypes.Structure):
+    """fg_tensor of include/featgraph_hip.h: one tensor of a list of gradients."""
+
+    _fields_ = [("data", _p), ("out", _p), ("n", _i64), ("dtype", _i32), ("reserved", _i32)]
+
 
 # name -> (restype, argtypes); mirrors include/featgraph_hip.h line by line
 SIGNATURES = {
@@ -55,6 +62,12 @@ SIGNATURES = {
     "fg_config_get": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(_i32)]),
     "fg_spmm_describe": (ctypes.c_int, [_p, _i32, _i32, _i32, ctypes.c_char_p, _i64]),
     "fg_sddmm_describe": (ctypes.c_int, [_i64, _i32, _i32, ctypes.c_char_p, _i64]),
+    "fg_embedding_lookup": (ctypes.c_int, [_i64, _i64, _i64, _p, _p, _p, _f32, _i32, _i32, _p]),
+    "fg_embedding_grad_workspace": (ctypes.c_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
+    "fg_embedding_grad": (ctypes.c_int, [_i64, _i64, _i64, _p, _p, _p, _f32, _i32, _i32, _i32, _p, _i64, _p]),
+    "fg_grad_norm_workspace": (ctypes.c_int, [ctypes.POINTER(_i64)]),
+    "fg_grad_norm": (ctypes.c_int, [_i32, ctypes.POINTER(Tensor), _p, _p, _i64, _p]),
+    "fg_grad_clip": (ctypes.c_int, [_i32, ctypes.POINTER(Tensor), _f32, _f32, _p, _p, _i64, _p]),
 }
 
 FG_EUNSUPPORTED = -4   # include/featgraph_hip.h

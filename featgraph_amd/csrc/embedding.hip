@@ -1,0 +1,601 @@
+// Embedding lookup with scaling, and its gradient.
+//
+//   lookup     out[i, :]   = scale * table[id[i], :]
+//   gradient   grad[v, :]  = scale * sum over i with id[i] = v of dout[i, :]
+//
+// An id outside [0, V) is padding: its output row is zero and it adds nothing to the gradient.  Sums are held in
+// float32 and rounded once to the element type.
+//
+// The gradient is a sum over runs of a sorted list, so that no atomic decides an order: the positions are sorted by
+// id (stably, so equal ids keep their order), the sorted list is cut into chunks, a group of lanes walks each chunk
+// and adds the rows of each run.  A run inside one chunk is written out at once; of a run that crosses a chunk's
+// border each chunk leaves a partial row (at most two per chunk: its first and its last run), and the partial rows,
+// again a sorted list, are added the same way.  The order of every sum depends on the ids and the sizes alone.
+#include <algorithm>
+#include <initializer_list>
+
+#include "element.hpp"
+
+namespace fg {
+namespace {
+
+constexpr int kRankSortMost = 8192;   // ids that the one-launch sort takes (32 KB of LDS)
+constexpr int kRadixItems = 2048;     // ids per workgroup of the radix sort
+constexpr int kRadixBits = 11;        // most bits per pass
+constexpr int32_t kSkip = INT32_MIN;  // flag on a partial row's key: nothing there to add
+
+int lanes_per_row(int64_t D, int vec) {
+  int l = 1;
+  while (l < kWaveSize && static_cast<int64_t>(l) * vec < D) l <<= 1;
+  return l;
+}
+
+template <typename Id>
+__device__ __forceinline__ int32_t key_of(Id id, int32_t V) {
+  return id >= 0 && id < static_cast<Id>(V) ? static_cast<int32_t>(id) : V;
+}
+
+// ------------------------------------------------------------------------------------------------ lookup
+// A group of lpr lanes copies kRows rows at a time, each lane VEC elements of each: all ids first, then all rows,
+// so that kRows gathers are in flight per lane.
+template <typename T, typename Id, int VEC>
+__global__ __launch_bounds__(kBlockThreads) void lookup_kernel(const T *table, const Id *ids, T *out, int64_t n,
+                                                               int32_t V, int32_t D, int lpr, float scale) {
+  constexpr int kRows = 4;
+  using P = Pack<T, VEC>;
+  const int sub = threadIdx.x & (lpr - 1);
+  const int64_t group = (static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x) / lpr;
+  const int64_t first = group * kRows;
+  if (first >= n) return;
+  int32_t key[kRows];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) key[r] = first + r < n ? key_of<Id>(ids[first + r], V) : V;
+  for (int32_t c = (blockIdx.y * lpr + sub) * VEC; c < D; c += gridDim.y * lpr * VEC) {
+    P x[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (key[r] < V) x[r] = *reinterpret_cast<const P *>(table + static_cast<int64_t>(key[r]) * D + c);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      if (first + r >= n) break;
+      P y;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) y.v[k] = key[r] < V ? narrow<T>(widen(x[r].v[k]) * scale) : narrow<T>(0.0f);
+      *reinterpret_cast<P *>(out + (first + r) * D + c) = y;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+// Up to kRankSortMost ids: the place of id i is the number of ids below it plus the number of equal ids before it,
+// counted directly.  A workgroup holds all ids in LDS and places 64 of them; each of its four waves counts over a
+// quarter of the list, four ids per LDS read.  N * N / 64 wave steps, but one launch.
+template <typename Id>
+__global__ __launch_bounds__(kBlockThreads) void rank_sort_kernel(const Id *ids, int32_t n, int32_t V, int32_t *keys,
+                                                                  int32_t *pos) {
+  __shared__ int4 all[kRankSortMost / 4];
+  __shared__ int32_t count[kWavesPerBlock][kWaveSize];
+  int32_t *flat = reinterpret_cast<int32_t *>(all);
+  const int padded = (n + 15) & ~15;
+  for (int j = threadIdx.x; j < padded; j += kBlockThreads) flat[j] = j < n ? key_of<Id>(ids[j], V) : INT32_MAX;
+  __syncthreads();
+  const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
+  const int base = blockIdx.x * kWaveSize, i = base + lane;
+  const int32_t mine = i < n ? flat[i] : -1;
+  const int quads = padded / 4, share = quads / kWavesPerBlock;
+  int32_t below = 0;
+  int q = wave * share;
+  const int end = q + share;
+  for (; q < min(end, base / 4); ++q) {  // ids before this workgroup's: equal ones count
+    const int4 k = all[q];
+    below += (k.x <= mine) + (k.y <= mine) + (k.z <= mine) + (k.w <= mine);
+  }
+  for (; q < min(end, (base + kWaveSize) / 4); ++q) {
+    const int4 k = all[q];
+    const int j = q * 4;
+    below += (k.x < mine || (k.x == mine && j < i)) + (k.y < mine || (k.y == mine && j + 1 < i)) +
+             (k.z < mine || (k.z == mine && j + 2 < i)) + (k.w < mine || (k.w == mine && j + 3 < i));
+  }
+  for (; q < end; ++q) {
+    const int4 k = all[q];
+    below += (k.x < mine) + (k.y < mine) + (k.z < mine) + (k.w < mine);
+  }
+  count[wave][lane] = below;
+  __syncthreads();
+  if (wave == 0 && i < n) {
+    const int place = count[0][lane] + count[1][lane] + count[2][lane] + count[3][lane];
+    keys[place] = mine;
+    pos[place] = i;
+  }
+}
+
+// More ids: least-significant-digit radix sort, digits of up to kRadixBits bits (two passes up to 4M rows), three
+// launches per pass: counts per workgroup and digit, a scan of each digit's counts over the workgroups, the scatter.
+template <typename Id>
+__global__ __launch_bounds__(kBlockThreads) void radix_count_kernel(const Id *keys, int32_t n, int32_t V, int shift,
+                                                                    int bits, int32_t *counts) {
+  __shared__ int32_t hist[1 << kRadixBits];
+  const int digits = 1 << bits;
+  for (int d = threadIdx.x; d < digits; d += kBlockThreads) hist[d] = 0;
+  __syncthreads();
+  const int32_t lo = blockIdx.x * kRadixItems;
+#pragma unroll
+  for (int r = 0; r < kRadixItems / kBlockThreads; ++r) {
+    const int64_t i = static_cast<int64_t>(lo) + r * kBlockThreads + threadIdx.x;
+    if (i < n) atomicAdd(&hist[(key_of<Id>(keys[i], V) >> shift) & (digits - 1)], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < digits; d += kBlockThreads)
+    counts[static_cast<int64_t>(d) * gridDim.x + blockIdx.x] = hist[d];
+}
+
+// One wave per digit: exclusive scan of its counts over the workgroups, in place, and their total.
+__global__ __launch_bounds__(kBlockThreads) void radix_scan_kernel(int32_t *counts, int32_t blocks, int32_t digits,
+                                                                   int32_t *totals) {
+  const int lane = threadIdx.x & (kWaveSize - 1);
+  const int d = blockIdx.x * kWavesPerBlock + threadIdx.x / kWaveSize;
+  if (d >= digits) return;
+  int32_t *c = counts + static_cast<int64_t>(d) * blocks;
+  int32_t before = 0;
+  for (int32_t b = 0; b < blocks; b += kWaveSize) {
+    const int32_t x = b + lane < blocks ? c[b + lane] : 0;
+    int32_t s = x;
+#pragma unroll
+    for (int k = 1; k < kWaveSize; k <<= 1) {
+      const int32_t y = __shfl_up(s, k, kWaveSize);
+      if (lane >= k) s += y;
+    }
+    if (b + lane < blocks) c[b + lane] = before + s - x;
+    before += __shfl(s, kWaveSize - 1, kWaveSize);
+  }
+  if (lane == 0) totals[d] = before;
+}
+
+// A wave ranks its consecutive kRadixItems / 4 keys, 64 at a time: lanes of equal digit find each other by one ballot
+// per bit, the first of them takes their places from the wave's counter of that digit.
+template <typename Id, bool kFirst>
+__global__ __launch_bounds__(kBlockThreads) void radix_scatter_kernel(const Id *keys, const int32_t *pos, int32_t n,
+                                                                      int32_t V, int shift, int bits,
+                                                                      const int32_t *counts, const int32_t *totals,
+                                                                      int32_t *keys_out, int32_t *pos_out) {
+  constexpr int kMost = 1 << kRadixBits, kRounds = kRadixItems / kBlockThreads;
+  __shared__ int32_t taken[kWavesPerBlock][kMost];  // per wave and digit: keys ranked so far
+  __shared__ int32_t base[kMost];                   // first place of each digit for this workgroup
+  __shared__ int32_t sums[kBlockThreads];
+  const int digits = 1 << bits, lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
+  for (int d = threadIdx.x; d < digits; d += kBlockThreads) {
+    base[d] = totals[d];
+#pragma unroll
+    for (int w = 0; w < kWavesPerBlock; ++w) taken[w][d] = 0;
+  }
+  __syncthreads();
+  {  // exclusive scan of the totals over the digits: each thread owns `per` neighbouring digits
+    const int per = (digits + kBlockThreads - 1) / kBlockThreads, d0 = threadIdx.x * per;
+    int32_t s = 0;
+    for (int k = 0; k < per; ++k) s += d0 + k < digits ? base[d0 + k] : 0;
+    sums[threadIdx.x] = s;
+    __syncthreads();
+    for (int k = 1; k < kBlockThreads; k <<= 1) {
+      const int32_t y = static_cast<int>(threadIdx.x) >= k ? sums[threadIdx.x - k] : 0;
+      __syncthreads();
+      sums[threadIdx.x] += y;
+      __syncthreads();
+    }
+    int32_t before = threadIdx.x ? sums[threadIdx.x - 1] : 0;
+    for (int k = 0; k < per; ++k) {
+      if (d0 + k >= digits) break;
+      const int32_t x = base[d0 + k];
+      base[d0 + k] = before + counts[static_cast<int64_t>(d0 + k) * gridDim.x + blockIdx.x];
+      before += x;
+    }
+  }
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kRadixItems + wave * (kRadixItems / kWavesPerBlock);
+  int32_t key[kRounds], from[kRounds], rank[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = lo + r * kWaveSize + lane;
+    key[r] = i < n ? key_of<Id>(keys[i], V) : 0;
+    from[r] = i < n ? (kFirst ? static_cast<int32_t>(i) : pos[i]) : -1;
+  }
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int d = (key[r] >> shift) & (digits - 1);
+    uint64_t peers = __ballot(from[r] >= 0);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1);
+      peers &= (d >> b) & 1 ? set : ~set;
+    }
+    const int leader = peers ? __ffsll(static_cast<unsigned long long>(peers)) - 1 : lane;
+    int32_t old = 0;
+    if (from[r] >= 0 && lane == leader) old = atomicAdd(&taken[wave][d], __popcll(peers));
+    rank[r] = __shfl(old, leader, kWaveSize) + __popcll(peers & ((uint64_t{1} << lane) - 1));
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    if (from[r] < 0) continue;
+    const int d = (key[r] >> shift) & (digits - 1);
+    int32_t place = base[d] + rank[r];
+    for (int w = 0; w < wave; ++w) place += taken[w][d];
+    keys_out[place] = key[r];
+    pos_out[place] = from[r];
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sums over runs
+template <typename T, int VEC>
+__device__ __forceinline__ void write_row(T *grad, int64_t at, const float *acc, float scale, int accumulate) {
+  using P = Pack<T, VEC>;
+  P y;
+  if (accumulate) {
+    y = *reinterpret_cast<const P *>(grad + at);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) y.v[k] = narrow<T>(__builtin_fmaf(acc[k], scale, widen(y.v[k])));
+  } else {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) y.v[k] = narrow<T>(acc[k] * scale);
+  }
+  *reinterpret_cast<P *>(grad + at) = y;
+}
+
+struct RunArgs {
+  const int32_t *keys;  // [n] ascending (partial rows: with kSkip set where there is nothing to add)
+  const int32_t *pos;   // [n] row of each entry (null: the entry's own place)
+  int64_t n;
+  int32_t chunk;        // entries per group
+  int32_t V, D;
+  int lpr, accumulate;
+  float scale;
+  float *part;          // [2 * chunks, D] partial rows, slots 2c and 2c + 1 for the first and last run of chunk c
+  int32_t *part_keys;   // [2 * chunks]
+};
+
+// S: element type of the rows that are added (the gradient's own, or float for partial rows).
+template <typename S, typename T, int VEC>
+__global__ __launch_bounds__(kBlockThreads) void run_sums_kernel(RunArgs a, const S *rows, T *grad) {
+  constexpr int kAhead = 4;
+  using P = Pack<S, VEC>;
+  const int sub = threadIdx.x & (a.lpr - 1);
+  const int64_t c = (static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x) / a.lpr;
+  const int64_t lo = c * a.chunk, hi = min(lo + a.chunk, a.n);
+  if (lo >= a.n) return;
+  const int32_t col = (blockIdx.y * a.lpr + sub) * VEC;
+  const bool mine = col < a.D, keeper = blockIdx.y == 0 && sub == 0;
+  const int32_t prev = lo > 0 ? a.keys[lo - 1] & ~kSkip : -1, next = hi < a.n ? a.keys[hi] & ~kSkip : -1;
+  int32_t cur = a.keys[lo] & ~kSkip;
+  const int32_t first_key = cur;
+  bool first = true, any = false, head = false, tail = false;  // head / tail: the two slots hold something
+  float acc[VEC] = {};
+  auto flush = [&](bool last) {
+    const bool whole = !(first && prev == cur) && !(last && next == cur);
+    if (any) {
+      if (whole) {
+        if (mine) write_row<T, VEC>(grad, static_cast<int64_t>(cur) * a.D + col, acc, a.scale, a.accumulate);
+      } else {
+        (first ? head : tail) = true;
+        if (mine) {
+          float *p = a.part + (2 * c + (first ? 0 : 1)) * a.D + col;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) p[k] = acc[k];
+        }
+      }
+    }
+  };
+  for (int64_t e = lo; e < hi; e += kAhead) {
+    int32_t key[kAhead];
+    P x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) key[u] = e + u < hi ? a.keys[e + u] : a.V;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (key[u] >= 0 && key[u] < a.V && mine) {
+        const int64_t r = a.pos ? a.pos[e + u] : e + u;
+        x[u] = *reinterpret_cast<const P *>(rows + r * a.D + col);
+      }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (e + u >= hi) break;
+      const int32_t k = key[u] & ~kSkip;
+      if (k != cur) {
+        flush(false);
+        cur = k;
+        first = any = false;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] = 0.0f;
+      }
+      if (key[u] >= 0 && key[u] < a.V) {
+        any = true;
+        if (mine) {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) acc[j] += widen(x[u].v[j]);
+        }
+      }
+    }
+  }
+  flush(true);
+  if (keeper) {
+    a.part_keys[2 * c] = first_key | (head ? 0 : kSkip);
+    a.part_keys[2 * c + 1] = cur | (tail ? 0 : kSkip);
+  }
+}
+
+// The last level: the group at a run's first entry adds the whole run.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kBlockThreads) void run_join_kernel(RunArgs a, const float *rows, T *grad) {
+  const int sub = threadIdx.x & (a.lpr - 1);
+  const int64_t e0 = (static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x) / a.lpr;
+  if (e0 >= a.n) return;
+  const int32_t k = a.keys[e0] & ~kSkip;
+  if (k >= a.V || (e0 > 0 && (a.keys[e0 - 1] & ~kSkip) == k)) return;
+  const int32_t col = (blockIdx.y * a.lpr + sub) * VEC;
+  if (col >= a.D) return;
+  float acc[VEC] = {};
+  bool any = false;
+  for (int64_t e = e0; e < a.n; ++e) {
+    const int32_t key = a.keys[e];
+    if ((key & ~kSkip) != k) break;
+    if (key < 0) continue;
+    any = true;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) acc[j] += rows[e * a.D + col + j];
+  }
+  if (any) write_row<T, VEC>(grad, static_cast<int64_t>(k) * a.D + col, acc, a.scale, a.accumulate);
+}
+
+// Zeros in the rows that no id names.  A wave looks 64 rows up in the sorted ids (one binary search per lane), then
+// writes those of them that are absent.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kBlockThreads) void zero_absent_kernel(const int32_t *keys, int32_t n, int32_t V,
+                                                                    int32_t D, int lpr, T *grad) {
+  using P = Pack<T, VEC>;
+  const int lane = threadIdx.x & (kWaveSize - 1), sub = lane & (lpr - 1);
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWaveSize) * kWaveSize;
+  if (r0 >= V) return;
+  int32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int32_t m = lo + (hi - lo) / 2;
+    if (keys[m] < r0 + lane) lo = m + 1; else hi = m;
+  }
+  const uint64_t present = __ballot(lo < n && keys[lo] == r0 + lane);
+  P z;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) z.v[k] = narrow<T>(0.0f);
+  for (int r = lane / lpr; r < kWaveSize && r0 + r < V; r += kWaveSize / lpr) {
+    if ((present >> r) & 1) continue;
+    for (int32_t c = sub * VEC; c < D; c += lpr * VEC) *reinterpret_cast<P *>(grad + (r0 + r) * D + c) = z;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host side
+int64_t align256(int64_t b) { return (b + 255) & ~int64_t{255}; }
+
+// Entries per group on the first level: short chunks where the list is short (more groups in flight), longer ones
+// where it is long (fewer partial rows).
+int32_t chunk_of(int64_t n) { return n <= 65536 ? 16 : n <= 524288 ? 32 : 64; }
+constexpr int32_t kSecondChunk = 64;
+constexpr int64_t kJoinMost = 512;  // partial rows from which a second level runs before the join
+
+struct GradLayout {
+  int64_t keys[2], pos[2], counts, totals, part1, part1_keys, part2, part2_keys, bytes;
+  int64_t chunks1, chunks2;
+};
+
+GradLayout grad_layout(int64_t n, int64_t D) {
+  GradLayout g;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  g.chunks1 = (n + chunk_of(n) - 1) / chunk_of(n);
+  const int64_t e2 = 2 * g.chunks1;
+  g.chunks2 = e2 > kJoinMost ? (e2 + kSecondChunk - 1) / kSecondChunk : 0;
+  const int64_t blocks = (n + kRadixItems - 1) / kRadixItems;
+  for (int k = 0; k < 2; ++k) {
+    g.keys[k] = take(n * 4);
+    g.pos[k] = take(n * 4);
+  }
+  g.counts = take(n > kRankSortMost ? blocks * (int64_t{4} << kRadixBits) : 0);
+  g.totals = take(int64_t{4} << kRadixBits);
+  g.part1 = take(2 * g.chunks1 * D * 4);
+  g.part1_keys = take(2 * g.chunks1 * 4);
+  g.part2 = take(2 * g.chunks2 * D * 4);
+  g.part2_keys = take(2 * g.chunks2 * 4);
+  g.bytes = at;
+  return g;
+}
+
+unsigned blocks_for(int64_t groups, int lpr) {
+  const int64_t per = kBlockThreads / lpr;
+  return static_cast<unsigned>((groups + per - 1) / per);
+}
+
+template <typename Id>
+int sort_ids(const Id *ids, int32_t n, int32_t V, char *ws, const GradLayout &g, const int32_t **keys,
+             const int32_t **pos, hipStream_t stream) {
+  auto *k0 = reinterpret_cast<int32_t *>(ws + g.keys[0]), *k1 = reinterpret_cast<int32_t *>(ws + g.keys[1]);
+  auto *p0 = reinterpret_cast<int32_t *>(ws + g.pos[0]), *p1 = reinterpret_cast<int32_t *>(ws + g.pos[1]);
+  if (n <= kRankSortMost) {
+    rank_sort_kernel<Id><<<dim3((n + kWaveSize - 1) / kWaveSize), dim3(kBlockThreads), 0, stream>>>(ids, n, V, k0, p0);
+    FG_HIP_TRY(hipGetLastError());
+    *keys = k0;
+    *pos = p0;
+    return FG_OK;
+  }
+  int total_bits = 1;
+  while (total_bits < 31 && (V >> total_bits) != 0) ++total_bits;  // keys 0 .. V
+  const int passes = (total_bits + kRadixBits - 1) / kRadixBits, bits = (total_bits + passes - 1) / passes;
+  const int32_t blocks = static_cast<int32_t>((static_cast<int64_t>(n) + kRadixItems - 1) / kRadixItems);
+  auto *counts = reinterpret_cast<int32_t *>(ws + g.counts), *totals = reinterpret_cast<int32_t *>(ws + g.totals);
+  for (int p = 0; p < passes; ++p) {
+    const int shift = p * bits;
+    if (p == 0)
+      radix_count_kernel<Id><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(ids, n, V, shift, bits, counts);
+    else
+      radix_count_kernel<int32_t><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(k0, n, V, shift, bits, counts);
+    radix_scan_kernel<<<dim3(((1 << bits) + kWavesPerBlock - 1) / kWavesPerBlock), dim3(kBlockThreads), 0, stream>>>(
+        counts, blocks, 1 << bits, totals);
+    if (p == 0)
+      radix_scatter_kernel<Id, true><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(ids, nullptr, n, V, shift, bits,
+                                                                                       counts, totals, k1, p1);
+    else
+      radix_scatter_kernel<int32_t, false><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(
+          k0, p0, n, V, shift, bits, counts, totals, k1, p1);
+    std::swap(k0, k1);
+    std::swap(p0, p1);
+  }
+  FG_HIP_TRY(hipGetLastError());
+  *keys = k0;
+  *pos = p0;
+  return FG_OK;
+}
+
+template <typename T, int VEC>
+int grad_rows(const int32_t *keys, const int32_t *pos, int64_t n, int64_t V, int64_t D, const T *dout, T *grad,
+              float scale, int accumulate, char *ws, const GradLayout &g, hipStream_t stream) {
+  const int lpr = lanes_per_row(D, VEC);
+  const unsigned tiles = static_cast<unsigned>((D + lpr * VEC - 1) / (lpr * VEC));
+  if (!accumulate) {
+    const int64_t waves = (V + kWaveSize - 1) / kWaveSize;
+    zero_absent_kernel<T, VEC><<<dim3(static_cast<unsigned>((waves + kWavesPerBlock - 1) / kWavesPerBlock)),
+                                 dim3(kBlockThreads), 0, stream>>>(keys, static_cast<int32_t>(n),
+                                                                   static_cast<int32_t>(V), static_cast<int32_t>(D),
+                                                                   lpr, grad);
+  }
+  if (n == 0) {
+    FG_HIP_TRY(hipGetLastError());
+    return FG_OK;
+  }
+  RunArgs a{};
+  a.keys = keys;
+  a.pos = pos;
+  a.n = n;
+  a.chunk = chunk_of(n);
+  a.V = static_cast<int32_t>(V);
+  a.D = static_cast<int32_t>(D);
+  a.lpr = lpr;
+  a.accumulate = accumulate;
+  a.scale = scale;
+  a.part = reinterpret_cast<float *>(ws + g.part1);
+  a.part_keys = reinterpret_cast<int32_t *>(ws + g.part1_keys);
+  run_sums_kernel<T, T, VEC><<<dim3(blocks_for(g.chunks1, lpr), tiles), dim3(kBlockThreads), 0, stream>>>(a, dout, grad);
+  const float *rows = a.part;
+  a.keys = a.part_keys;
+  a.pos = nullptr;
+  a.n = 2 * g.chunks1;
+  if (g.chunks2) {
+    a.chunk = kSecondChunk;
+    a.part = reinterpret_cast<float *>(ws + g.part2);
+    a.part_keys = reinterpret_cast<int32_t *>(ws + g.part2_keys);
+    run_sums_kernel<float, T, VEC><<<dim3(blocks_for(g.chunks2, lpr), tiles), dim3(kBlockThreads), 0, stream>>>(a, rows, grad);
+    rows = a.part;
+    a.keys = a.part_keys;
+    a.n = 2 * g.chunks2;
+  }
+  run_join_kernel<T, VEC><<<dim3(blocks_for(a.n, lpr), tiles), dim3(kBlockThreads), 0, stream>>>(a, rows, grad);
+  FG_HIP_TRY(hipGetLastError());
+  return FG_OK;
+}
+
+template <typename T>
+int grad_typed(const int32_t *keys, const int32_t *pos, int64_t n, int64_t V, int64_t D, const void *dout, void *grad,
+               float scale, int accumulate, char *ws, const GradLayout &g, hipStream_t stream) {
+  const T *d = static_cast<const T *>(dout);
+  T *o = static_cast<T *>(grad);
+  switch (vector_elements(D, sizeof(T), {dout, grad})) {
+    case 8:
+      if constexpr (sizeof(T) == 2) return grad_rows<T, 8>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
+      [[fallthrough]];
+    case 4: return grad_rows<T, 4>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
+    case 2: return grad_rows<T, 2>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
+    default: return grad_rows<T, 1>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
+  }
+}
+
+template <typename T, typename Id>
+int lookup_typed(const void *table, const void *ids, void *out, int64_t n, int64_t V, int64_t D, float scale,
+                 hipStream_t stream) {
+  const T *t = static_cast<const T *>(table);
+  const Id *i = static_cast<const Id *>(ids);
+  T *o = static_cast<T *>(out);
+  const int vec = vector_elements(D, sizeof(T), {table, out}), lpr = lanes_per_row(D, vec);
+  const dim3 grid(blocks_for((n + 3) / 4, lpr),
+                  static_cast<unsigned>(std::min<int64_t>(16, (D + lpr * vec - 1) / (lpr * vec))));
+#define FG_LOOKUP(VEC)                                                                                          \
+  lookup_kernel<T, Id, VEC><<<grid, dim3(kBlockThreads), 0, stream>>>(t, i, o, n, static_cast<int32_t>(V),      \
+                                                                      static_cast<int32_t>(D), lpr, scale)
+  if constexpr (sizeof(T) == 2) {
+    if (vec == 8) FG_LOOKUP(8);
+  }
+  if (vec == 4) FG_LOOKUP(4);
+  if (vec == 2) FG_LOOKUP(2);
+  if (vec == 1) FG_LOOKUP(1);
+#undef FG_LOOKUP
+  FG_HIP_TRY(hipGetLastError());
+  return FG_OK;
+}
+
+// Sizes shared by the entry points: rows and columns that int32 counts, ids that int32 places.
+int check_sizes(int64_t V, int64_t D, int64_t n, int32_t dtype, int32_t itype) {
+  if (V < 1 || V >= 0x7fffffffLL) return fail(FG_EINVAL, "n_rows = %lld is out of range", (long long)V);
+  if (D < 1 || D > (1 << 20)) return fail(FG_EINVAL, "D = %lld is out of range", (long long)D);
+  if (n < 0 || n > 0x7fff0000LL) return fail(FG_EINVAL, "n_ids = %lld is out of range", (long long)n);
+  if (!element_type_ok(dtype)) return fail(FG_EINVAL, "dtype code %d is unknown", dtype);
+  if (!index_type_ok(itype)) return fail(FG_EINVAL, "index type code %d is unknown", itype);
+  return FG_OK;
+}
+
+}  // namespace
+}  // namespace fg
+
+extern "C" {
+
+int fg_embedding_lookup(int64_t n_rows, int64_t D, int64_t n_ids, const void *table, const void *ids, void *out,
+                        float scale, int32_t dtype, int32_t itype, void *stream) {
+  if (int rc = fg::check_sizes(n_rows, D, n_ids, dtype, itype)) return rc;
+  if (n_ids == 0) return FG_OK;
+  if (!table || !ids || !out) return fg::fail(FG_EINVAL, "a data pointer is null");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+#define FG_TYPED(T)                                                                                     \
+  (itype == FG_I32 ? fg::lookup_typed<T, int32_t>(table, ids, out, n_ids, n_rows, D, scale, s)          \
+                   : fg::lookup_typed<T, int64_t>(table, ids, out, n_ids, n_rows, D, scale, s))
+  if (dtype == FG_F32) return FG_TYPED(float);
+  if (dtype == FG_BF16) return FG_TYPED(__bf16);
+  return FG_TYPED(_Float16);
+#undef FG_TYPED
+}
+
+int fg_embedding_grad_workspace(int64_t n_rows, int64_t D, int64_t n_ids, int64_t *bytes) {
+  if (int rc = fg::check_sizes(n_rows, D, n_ids, FG_F32, FG_I32)) return rc;
+  if (!bytes) return fg::fail(FG_EINVAL, "bytes is null");
+  *bytes = fg::grad_layout(n_ids, D).bytes;
+  return FG_OK;
+}
+
+int fg_embedding_grad(int64_t n_rows, int64_t D, int64_t n_ids, const void *ids, const void *dout, void *grad,
+                      float scale, int32_t accumulate, int32_t dtype, int32_t itype, void *workspace,
+                      int64_t workspace_bytes, void *stream) {
+  if (int rc = fg::check_sizes(n_rows, D, n_ids, dtype, itype)) return rc;
+  if (n_ids == 0 && accumulate) return FG_OK;
+  const fg::GradLayout g = fg::grad_layout(n_ids, D);
+  if (!grad || (n_ids > 0 && (!ids || !dout))) return fg::fail(FG_EINVAL, "a data pointer is null");
+  if (!workspace || !fg::aligned_to(workspace, 256) || workspace_bytes < g.bytes)
+    return fg::fail(FG_EINVAL, "the workspace needs %lld bytes at a multiple of 256", (long long)g.bytes);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char *ws = static_cast<char *>(workspace);
+  const int32_t *keys = reinterpret_cast<const int32_t *>(ws), *pos = keys;
+  if (n_ids > 0) {
+    const int32_t n = static_cast<int32_t>(n_ids), V = static_cast<int32_t>(n_rows);
+    const int rc = itype == FG_I32 ? fg::sort_ids(static_cast<const int32_t *>(ids), n, V, ws, g, &keys, &pos, s)
+                                   : fg::sort_ids(static_cast<const int64_t *>(ids), n, V, ws, g, &keys, &pos, s);
+    if (rc) return rc;
+  }
+#define FG_TYPED(T) fg::grad_typed<T>(keys, pos, n_ids, n_rows, D, dout, grad, scale, accumulate, ws, g, s)
+  if (dtype == FG_F32) return FG_TYPED(float);
+  if (dtype == FG_BF16) return FG_TYPED(__bf16);
+  return FG_TYPED(_Float16);
+#undef FG_TYPED
+}
+
+}  // extern "C"

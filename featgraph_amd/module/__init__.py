@@ -6,3 +6,5 @@ from .attention import MultiHeadAttentionhip
 from .general import MultiHeadGeneralizedSpMMhip
 from .backward import (EdgeSoftmaxGradhip, MultiHeadAttentionGradhip, MultiHeadSDDMMGradhip,
                        MultiHeadSpMMGradhip)
+from .embedding import EmbeddingLookuphip, EmbeddingLookupGradhip
+from .grad_norm import ClipGradNormhip, GradNormhip

@@ -1,9 +1,11 @@
 """Host-side checks and helpers shared by the SpMM and SDDMM module classes."""
+import ctypes
+
 import numpy as np
 import torch
 
 from .. import _lib
-from ..runtime import as_tensor
+from ..runtime import as_tensor, hip
 
 INT32_MAX = 2 ** 31 - 1
 
@@ -81,3 +83,91 @@ def time_calls(fn, device, num_runs):
     stop.record(torch.cuda.current_stream(device))
     stop.synchronize()
     return start.elapsed_time(stop) * 1e-3 / num_runs
+
+
+# Element and index types of the training operators: (torch type, code of include/featgraph_hip.h).
+ELEMENT_TYPES = {"float32": (torch.float32, 0), "bfloat16": (torch.bfloat16, 1), "float16": (torch.float16, 2)}
+INDEX_TYPES = {"int32": (torch.int32, 0), "int64": (torch.int64, 1)}
+
+
+def typed(dtype, table, what):
+    """(torch type, code) of a placeholder's dtype, which must be one of `table`."""
+    try:
+        return table[str(dtype)]
+    except KeyError:
+        raise TypeError("%s must be one of %s, got %s" % (what, "/".join(table), dtype)) from None
+
+
+def check_typed_operand(x, shape, dtype, device, what):
+    """Device tensor of the built shape and type, dense row-major."""
+    t = as_tensor(x)
+    if t.device != device:
+        raise ValueError("%s lives on %s, the module on %s" % (what, t.device, device))
+    if t.dtype != dtype:
+        raise TypeError("%s must be %s, got %s" % (what, dtype, t.dtype))
+    if t.shape != shape:
+        raise ValueError("%s has shape %s, the module was built for %s" % (what, tuple(t.shape), tuple(shape)))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous (row-major)" % what)
+    return t
+
+
+def check_apart(written, read, what):
+    """A kernel writes `written` while it reads the tensors of `read`: no byte may be in both."""
+    lo = written.data_ptr()
+    hi = lo + written.numel() * written.element_size()
+    for t in read:
+        at = t.data_ptr()
+        if at < hi and lo < at + t.numel() * t.element_size():
+            raise ValueError("%s overlaps an operand of the same call" % what)
+
+
+class DenseBase:
+    """What the modules without an adjacency matrix share: the device, run() over checked operands, timing."""
+
+    _target = "hip"
+
+    def __init__(self):
+        require_device()
+        self._ctx = hip(0)
+        self._built = False
+        self.out_tvm = None
+
+    def _checked(self, arrays):
+        raise NotImplementedError
+
+    def _launch(self, tensors):
+        raise NotImplementedError
+
+    def run(self, input_tvm_ndarrays):
+        if not self._built:
+            raise RuntimeError("call build() before run()")
+        tensors = self._checked(input_tvm_ndarrays)
+        if torch.cuda.current_device() == self._ctx.index:
+            return self._launch(tensors)
+        with torch.cuda.device(self._ctx):
+            return self._launch(tensors)
+
+    def measure_average_time(self, input_tvm_ndarrays, num_runs):
+        if not self._built:
+            raise RuntimeError("call build() before measure_average_time()")
+        tensors = self._checked(input_tvm_ndarrays)
+        with torch.cuda.device(self._ctx):
+            return time_calls(lambda: self._launch(tensors), self._ctx, num_runs)
+
+    def _stream(self):
+        return torch.cuda.current_stream(self._ctx).cuda_stream
+
+    def _workspace(self, entry, *sizes):
+        """A workspace of the size that the library's `entry` gives, kept by the module."""
+        need = ctypes.c_int64(0)
+        _lib.check(getattr(_lib.lib(), entry)(*sizes, ctypes.byref(need)))
+        return torch.empty(max(256, need.value), dtype=torch.uint8, device=self._ctx)
+
+    @property
+    def ctx(self):
+        return self._ctx
+
+    @property
+    def target(self):
+        return self._target

@@ -57,8 +57,9 @@ class NDArray:
         return self.tensor.device
 
     def asnumpy(self):
-        """Copy to the host (synchronises with the device)."""
-        return self.tensor.detach().cpu().numpy()
+        """Copy to the host (synchronises with the device); bfloat16, which numpy lacks, as float32."""
+        t = self.tensor.detach()
+        return (t.float() if t.dtype == torch.bfloat16 else t).cpu().numpy()
 
     def __repr__(self):
         return "NDArray(shape=%s, dtype=%s, ctx=%s)" % (self.shape, self.dtype, self.ctx)

@@ -525,6 +525,70 @@ FG_API int fg_config_get(const char *key, int32_t *value);
 FG_API int fg_spmm_describe(const fg_spmm_plan *plan, int32_t H, int32_t D, int32_t feat_tiles, char *buf, int64_t cap);
 FG_API int fg_sddmm_describe(int64_t nnz, int32_t H, int32_t D, char *buf, int64_t cap);
 
+/* ------------------------------------------------------------------------
+ * The ends of a training step: learned vertex (entity) embeddings in, a loss
+ * over vertices or classes out, gradients clipped.  No counterparts in the
+ * reference, which has no learned parameters.
+ *
+ * Elements are float32, bfloat16 or float16 (dtype), ids and labels int32 or
+ * int64 (itype); all arrays dense row-major.  Every sum is held in float32 or
+ * more and rounded once to the element type.  Where a call takes a workspace
+ * it is caller-owned device memory at a multiple of 256 bytes, of the size its
+ * *_workspace function gives; its contents mean nothing between calls, and
+ * two calls that may overlap in time (two streams, two captured graphs) need
+ * one each.  The calls enqueue kernels only, so they can be captured.
+ * ------------------------------------------------------------------------ */
+#define FG_F32 0
+#define FG_BF16 1
+#define FG_F16 2
+#define FG_I32 0
+#define FG_I64 1
+
+/*
+ * out[i, :] = scale * table[ids[i], :] for table [n_rows, D] and out
+ * [n_ids, D].  An id outside [0, n_rows) is padding: its row becomes zero.
+ */
+FG_API int fg_embedding_lookup(int64_t n_rows, int64_t D, int64_t n_ids, const void *table, const void *ids, void *out,
+                               float scale, int32_t dtype, int32_t itype, void *stream);
+/*
+ * Its gradient: grad[v, :] = scale * sum over i with ids[i] = v of dout[i, :]
+ * (accumulate = 0: every row of grad [n_rows, D] is written, those that no id
+ * names with zeros), or grad[v, :] += the same (accumulate = 1: the other rows
+ * are not touched).  Padding ids add nothing, whatever their dout rows hold.
+ * Ids are sorted, equal ones keep their order, and rows are added along the
+ * sorted list: results do not depend on timing.  grad must not overlap dout.
+ */
+FG_API int fg_embedding_grad_workspace(int64_t n_rows, int64_t D, int64_t n_ids, int64_t *bytes);
+FG_API int fg_embedding_grad(int64_t n_rows, int64_t D, int64_t n_ids, const void *ids, const void *dout, void *grad,
+                             float scale, int32_t accumulate, int32_t dtype, int32_t itype, void *workspace,
+                             int64_t workspace_bytes, void *stream);
+
+/* One tensor of a list of gradients: n elements of type dtype at `in` (device). */
+typedef struct fg_tensor {
+  const void *in;
+  void *out; /* fg_grad_clip: n elements of the same type; may equal `in` */
+  int64_t n;
+  int32_t dtype;
+  int32_t reserved;
+} fg_tensor;
+
+/*
+ * *norm = sqrt of the sum of the squares of all elements of all tensors
+ * (device float).  `tensors` is HOST memory, read during the call.  Squares
+ * are added in float64.  Tensors without elements are legal.
+ */
+FG_API int fg_grad_norm_workspace(int64_t *bytes);
+FG_API int fg_grad_norm(int32_t count, const fg_tensor *tensors, float *norm, void *workspace, int64_t workspace_bytes,
+                        void *stream);
+/*
+ * The norm, and out = c * in for every tensor, c = min(1, max_norm / (norm + eps)).
+ * In place (out == in) nothing is written when c is 1.  A norm of NaN makes
+ * every element NaN, an infinite one makes finite elements 0, as the formula
+ * gives.  Distinct tensors must not overlap.
+ */
+FG_API int fg_grad_clip(int32_t count, const fg_tensor *tensors, float max_norm, float eps, float *norm, void *workspace,
+                        int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
