@@ -65,6 +65,10 @@ SIGNATURES = {
     "fg_embedding_lookup": (ctypes.c_int, [_i64, _i64, _i64, _p, _p, _p, _f32, _i32, _i32, _p]),
     "fg_embedding_grad_workspace": (ctypes.c_int, [_i64, _i64, _i64, ctypes.POINTER(_i64)]),
     "fg_embedding_grad": (ctypes.c_int, [_i64, _i64, _i64, _p, _p, _p, _f32, _i32, _i32, _i32, _p, _i64, _p]),
+    "fg_linear_ce_workspace": (ctypes.c_int, [_i64, _i64, _i64, _i32, ctypes.POINTER(_i64)]),
+    "fg_linear_ce": (ctypes.c_int, [_i64, _i64, _i64, _p, _p, _p, _p, _p, _i32, _i32, _p, _i64, _p]),
+    "fg_linear_ce_grad_workspace": (ctypes.c_int, [_i64, _i64, _i64, _i32, ctypes.POINTER(_i64)]),
+    "fg_linear_ce_grad": (ctypes.c_int, [_i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _p, _i64, _p]),
     "fg_grad_norm_workspace": (ctypes.c_int, [ctypes.POINTER(_i64)]),
     "fg_grad_norm": (ctypes.c_int, [_i32, ctypes.POINTER(Tensor), _p, _p, _i64, _p]),
     "fg_grad_clip": (ctypes.c_int, [_i32, ctypes.POINTER(Tensor), _f32, _f32, _p, _p, _i64, _p]),

@@ -446,6 +446,8 @@ int build_bounds(fg_spmm_plan *p) {
 int *config_slot(const char *key) {
   fg::Config &c = fg::config();
   if (!key) return nullptr;
+  if (!strcmp(key, "ce.tile")) return &c.ce_tile;
+  if (!strcmp(key, "ce.piece_rows")) return &c.ce_piece_rows;
   if (!strcmp(key, "spmm.vec")) return &c.spmm_vec;
   if (!strcmp(key, "spmm.lpr")) return &c.spmm_lpr;
   if (!strcmp(key, "spmm.unroll")) return &c.spmm_unroll;

@@ -8,3 +8,4 @@ from .backward import (EdgeSoftmaxGradhip, MultiHeadAttentionGradhip, MultiHeadS
                        MultiHeadSpMMGradhip)
 from .embedding import EmbeddingLookuphip, EmbeddingLookupGradhip
 from .grad_norm import ClipGradNormhip, GradNormhip
+from .cross_entropy import LinearCrossEntropyGradhip, LinearCrossEntropyhip

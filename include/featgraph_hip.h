@@ -510,7 +510,11 @@ FG_API int64_t fg_probe_gather_stream_f32(const float *feat, int32_t band_rows, 
  * not read it; default 1),
  * "attention.blocks" (grid size of the fused attention kernel; by default one
  * vertex row per wave when a row is 1 KB or more, else 65536 workgroups that
- * walk the rows).  Value 0 restores the default of a size; for the 0/1 flags a
+ * walk the rows), "ce.tile" (1..4: the 256 x 256, 128 x 128, 64 x 256 or 256 x 64
+ * tile for every product of fg_linear_ce and fg_linear_ce_grad), "ce.piece_rows"
+ * (vocabulary rows per piece of those calls, rounded up to a multiple of 256);
+ * both are read by the calls and by the functions that size their workspaces.
+ * Value 0 restores the default of a size; for the 0/1 flags a
  * negative value does.
  * The spmm.* keys change the launch shape only; "sddmm.group" and
  * "sddmm.rows_wide" also change the shape of the summation tree, i.e. the last
@@ -588,6 +592,36 @@ FG_API int fg_grad_norm(int32_t count, const fg_tensor *tensors, float *norm, vo
  */
 FG_API int fg_grad_clip(int32_t count, const fg_tensor *tensors, float max_norm, float eps, float *norm, void *workspace,
                         int64_t workspace_bytes, void *stream);
+
+/*
+ * Softmax cross entropy of a linear scorer over V classes (vertices, entities,
+ * a vocabulary) without keeping the N x V logits l[n, v] = <hidden[n], weight[v]>:
+ *   lse[n]  = log(sum over v of exp(l[n, v]))
+ *   loss[n] = lse[n] - l[n, labels[n]], 0 where the label is outside [0, V)
+ * for hidden [N, D] and weight [V, D] of float32 or bfloat16 (float16 returns
+ * FG_EUNSUPPORTED).  Logits, statistics and results are float32.  Limits:
+ * N <= 4194304, D <= 65536.
+ */
+FG_API int fg_linear_ce_workspace(int64_t N, int64_t V, int64_t D, int32_t dtype, int64_t *bytes);
+FG_API int fg_linear_ce(int64_t N, int64_t V, int64_t D, const void *hidden, const void *weight, const void *labels,
+                        float *loss, float *lse, int32_t dtype, int32_t itype, void *workspace, int64_t workspace_bytes,
+                        void *stream);
+/*
+ * Its gradients, for the lse of the forward call and the gradient dloss [N] of
+ * the losses:
+ *   G[n, v] = dloss[n] * (exp(l[n, v] - lse[n]) - [v = labels[n]])
+ *   dhidden[n, :] = sum over v of G[n, v] * weight[v, :]
+ *   dweight[v, :] = sum over n of G[n, v] * hidden[n, :]
+ * Rows whose label is outside [0, V) get zeros in dhidden and add nothing to
+ * dweight, whatever their hidden row, lse and dloss hold.  The logits are
+ * computed again, a piece of the vocabulary at a time.  With bfloat16 operands
+ * G is rounded to bfloat16; with float32 everything keeps float32's accuracy.
+ * dhidden and dweight must not overlap each other or an input.
+ */
+FG_API int fg_linear_ce_grad_workspace(int64_t N, int64_t V, int64_t D, int32_t dtype, int64_t *bytes);
+FG_API int fg_linear_ce_grad(int64_t N, int64_t V, int64_t D, const void *hidden, const void *weight, const void *labels,
+                             const float *lse, const float *dloss, void *dhidden, void *dweight, int32_t dtype,
+                             int32_t itype, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

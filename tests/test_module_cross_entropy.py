@@ -1,0 +1,305 @@
+"""Linear softmax cross entropy and its gradients against the formulas in 64 bits.
+
+Tolerances.  A sum of K float32 terms on the device differs from the exact one by K roundings, each at most half a
+step (2^-24) of a partial sum, which A = the sum of the terms' sizes bounds; roundings are of random sign, and six
+standard deviations of K of them are 6 * sqrt(K / 3) * 2^-24 * A < 4 * sqrt(K) * 2^-24 * A.  sums(K) below is that with
+room for the few roundings of partial joins; float32 operands, split into three bfloat16 parts, add 6 K products and
+leave out three of 2^-24 A at most.  A logit off by d moves exp by a factor 1 + d, lse by at most the largest d of its
+row, and G by |dloss| p (d + d_lse); exp2 of a product rounds its argument (|l - lse| 2^-23).  bfloat16 operands round G
+to bfloat16 (half a step, 2^-8), and the results are rounded to their type (half a step)."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from featgraph_amd import _lib, placeholder
+from featgraph_amd.module import LinearCrossEntropyGradhip, LinearCrossEntropyhip
+
+TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16}
+HALF_STEP = {"float32": 2.0 ** -24, "bfloat16": 2.0 ** -8}
+TINY = 2.0 ** -126
+
+
+def _operands(dtype, N, V, D, seed, spread=1.5, itype="int32", ignored=0.1):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(N, D, generator=g).to(TYPES[dtype]).cuda()
+    w = (torch.randn(V, D, generator=g) * (spread / math.sqrt(D))).to(TYPES[dtype]).cuda()
+    y = torch.randint(0, V, (N,), generator=g)
+    if N:
+        y[0] = V - 1
+    if N > 3:
+        y[torch.rand(N, generator=g) < ignored] = -1
+        y[2] = V                                             # one past the last class: ignored as well
+        y[1] = 0
+    dl = (0.5 + torch.rand(N, generator=g)).cuda() / max(N, 1)
+    return h, w, y.to(getattr(torch, itype)).cuda(), dl
+
+
+def _sums(K, dtype):
+    return (8 + 4 * math.sqrt(K * (6 if dtype == "float32" else 1)) + (3 if dtype == "float32" else 0)) * 2.0 ** -24
+
+
+def _reference(h, w, y, dl, dtype, loss, lse, dh, dw):
+    """Checks the four results against 64 bits."""
+    N, D = h.shape
+    V = w.shape[0]
+    H, W = h.double(), w.double()
+    logits, size = H @ W.T, H.abs() @ W.abs().T
+    d = (_sums(D, dtype) * size).amax(1)                      # of every logit of the row
+    want = torch.logsumexp(logits, 1)
+    far = (logits - want[:, None]).abs().amax(1)
+    d_lse = d + (far * 2.0 ** -23 + 2.0 ** -21) + _sums(V, "bfloat16") + 2.0 ** -23 * want.abs()
+    assert bool(((lse.double() - want).abs() <= d_lse).all())
+    ok = (y >= 0) & (y < V)
+    n = torch.arange(N, device="cuda")[ok]
+    at = y[ok].long()
+    want_loss = torch.zeros_like(want)
+    want_loss[ok] = want[ok] - logits[n, at]
+    tol = d_lse + d + 2.0 ** -23 * want_loss.abs()
+    assert bool(((loss.double() - want_loss).abs() <= tol).all()) and not loss[~ok].any()
+    if dh is None:
+        return
+    p = torch.exp(logits - want[:, None])
+    f = torch.where(ok, dl.double(), 0.0)[:, None]
+    G = p * f
+    G[n, at] -= dl.double()[ok]
+    off = f * (p * (d + d_lse + far * 2.0 ** -23 + 2.0 ** -21)[:, None] + 2.0 ** -22 * (p + 0.0))
+    off[n, at] += 2.0 ** -22 * dl.double()[ok]
+    rounding = 2.0 ** -8 if dtype == "bfloat16" else 3 * 2.0 ** -24
+    for got, a, b, K, e in ((dh, G, W, V, off), (dw, G.T, H, N, off.T)):
+        exact = a @ b
+        tol = (e + (rounding + _sums(K, dtype)) * a.abs()) @ b.abs() + HALF_STEP[dtype] * exact.abs() * 1.01 + TINY
+        assert bool(((got.double() - exact).abs() <= tol).all())
+    assert not dh[~ok].any()
+
+
+def _run(h, w, y, dl, dtype, itype="int32"):
+    ph = [placeholder(tuple(h.shape), dtype), placeholder(tuple(w.shape), dtype), placeholder(tuple(y.shape), itype)]
+    f, g = LinearCrossEntropyhip(), LinearCrossEntropyGradhip()
+    f.build(ph), g.build(ph)
+    loss, lse = f.run([h, w, y])
+    g._dhidden.tensor.fill_(float("nan")), g._dweight.tensor.fill_(float("nan"))
+    dh, dw = g.run([h, w, y, lse, dl])
+    return loss.tensor, lse.tensor, dh.tensor, dw.tensor
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("N,V,D", [(1, 1, 1), (5, 3, 2), (64, 41, 64), (127, 255, 100), (33, 300, 64), (300, 70, 130),
+                                   (257, 1025, 192), (70, 5000, 72), (1000, 41, 256), (20, 30001, 40), (1, 4096, 64),
+                                   (2049, 513, 24), (9, 1, 5)])
+def test_loss_and_gradients(dtype, N, V, D):
+    itype = "int64" if N % 2 else "int32"
+    h, w, y, dl = _operands(dtype, N, V, D, N + V + D, itype=itype)
+    loss, lse, dh, dw = _run(h, w, y, dl, dtype, itype)
+    assert loss.dtype == lse.dtype == torch.float32 and dh.dtype == dw.dtype == TYPES[dtype]
+    _reference(h, w, y, dl, dtype, loss, lse, dh, dw)
+
+
+@pytest.fixture
+def config():
+    yield _lib.config_set
+    _lib.config_set("ce.tile", 0)
+    _lib.config_set("ce.piece_rows", 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("N,V,D,piece", [(300, 700, 192, 0), (300, 700, 192, 256), (65, 1300, 70, 512), (600, 257, 128, 256)])
+def test_every_tile_and_pieces_of_the_vocabulary(config, dtype, tile, N, V, D, piece):
+    config("ce.tile", tile)
+    config("ce.piece_rows", piece)
+    h, w, y, dl = _operands(dtype, N, V, D, tile + N)
+    first = _run(h, w, y, dl, dtype)
+    _reference(h, w, y, dl, dtype, *first)
+    assert all(torch.equal(a, b) for a, b in zip(first, _run(h, w, y, dl, dtype)))      # the same bits again
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_steep_and_flat_logits(dtype):
+    h, w, y, dl = _operands(dtype, 130, 500, 64, 3, spread=200.0)      # logits of hundreds: the softmax is a maximum
+    _reference(h, w, y, dl, dtype, *_run(h, w, y, dl, dtype))
+    h.zero_()                                                          # all logits 0: lse = log V, G = 1 / V
+    loss, lse, dh, dw = _run(h, w, y, dl, dtype)
+    assert bool(((lse.double() - math.log(500)).abs() <= 2.0 ** -20).all())
+    _reference(h, w, y, dl, dtype, loss, lse, dh, dw)
+
+
+@pytest.mark.gpu
+def test_the_smallest_and_largest_values():
+    """float32 operands near the ends of the range: leading parts that would round to infinity are cut instead.  The
+    weights are powers of two, so that every part of every product is a normal number."""
+    h = torch.zeros(4, 8, device="cuda")
+    w = torch.zeros(5, 8, device="cuda")
+    h[0, 0], w[1, 0] = 3.4e38, 2.0 ** -125
+    h[1, 1], w[2, 1] = 1.2345678 * 2.0 ** -100, 2.0 ** 102
+    h[2, 2], w[3, 2] = -torch.finfo(torch.float32).max, 2.0 ** -126
+    y = torch.tensor([1, 2, 3, 4], dtype=torch.int32, device="cuda")
+    loss, lse, _, _ = _run(h, w, y, torch.ones(4, device="cuda"), "float32")
+    logits = h.double() @ w.double().T
+    want = torch.logsumexp(logits, 1)
+    tol = 40 * 2.0 ** -24 * (logits.abs().amax(1) + 4)                  # a dozen roundings of values up to the logit, exp, log
+    assert bool(((lse.double() - want).abs() <= tol).all())
+    at = logits[torch.arange(4, device="cuda"), y.long()]
+    assert bool(((loss.double() - (want - at)).abs() <= 2 * tol).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_ignored_rows_may_hold_anything(dtype):
+    h, w, y, dl = _operands(dtype, 200, 333, 96, 5, ignored=0.4)
+    bad = (y < 0) | (y >= 333)
+    ph = [placeholder((200, 96), dtype), placeholder((333, 96), dtype), placeholder((200,), "int32")]
+    f, g = LinearCrossEntropyhip(), LinearCrossEntropyGradhip()
+    f.build(ph), g.build(ph)
+    loss, lse = (x.tensor.clone() for x in f.run([h, w, y]))
+    dh, dw = (x.tensor.clone() for x in g.run([h, w, y, lse, dl]))
+    h[bad] = float("nan")
+    dl[bad] = float("inf")
+    loss2, lse2 = f.run([h, w, y])
+    assert torch.equal(loss2.tensor, loss) and torch.equal(lse2.tensor[~bad], lse[~bad])
+    dh2, dw2 = g.run([h, w, y, lse2, dl])
+    assert torch.equal(dh2.tensor, dh) and torch.equal(dw2.tensor, dw) and not dh2.tensor[bad].any()
+    y.fill_(-1)                                                        # nothing left
+    assert not f.run([h, w, y])[0].tensor.any()
+    dh3, dw3 = g.run([h, w, y, lse2, dl])
+    assert not dh3.tensor.any() and not dw3.tensor.any()
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """(L(x + e u) - L(x - e u)) / 2e for the summed loss L along a direction u.  Along it every logit moves linearly
+    (in h) with slope s; the third derivative of lse is at most 2 * max |s|^3 (a third cumulant of a variable within
+    [-max, max] is below 2 max^3), so the difference is off by e^2 / 6 of that, plus the losses' own error over e."""
+    N, V, D = 64, 300, 48
+    h, w, y, dl = _operands("float32", N, V, D, 7)
+    ph = [placeholder((N, D)), placeholder((V, D)), placeholder((N,), "int32")]
+    f, g = LinearCrossEntropyhip(), LinearCrossEntropyGradhip()
+    f.build(ph), g.build(ph)
+    ok = (y >= 0) & (y < V)
+    _, lse = f.run([h, w, y])
+    dh, dw = (x.tensor.double().clone() for x in g.run([h, w, y, lse, dl]))
+    gen = torch.Generator().manual_seed(8)
+    loss_error = 4 * float((_sums(D, "float32") * (h.double().abs() @ w.double().abs().T)).max()) + 2.0 ** -18
+    for which in (0, 1):
+        u = torch.randn(*(h, w)[which].shape, generator=gen).cuda() / math.sqrt(D)
+        slopes = (u.double() @ w.double().T) if which == 0 else (h.double() @ u.double().T)
+        e = 1.0 / 64
+        sides = []
+        for sign in (1, -1):
+            x = [h, w]
+            x[which] = x[which] + sign * e * u
+            sides.append((f.run([x[0], x[1], y])[0].tensor.double() * dl.double())[ok].sum())
+            real = (x[which] - (h, w)[which]).double()
+            sides[-1] = (sides[-1], real)
+        step = (sides[0][1] - sides[1][1])                              # what the sums in float32 really moved by
+        want = float((step * (dh, dw)[which]).sum())
+        got = float(sides[0][0] - sides[1][0])
+        total = float(dl[ok].sum())
+        bound = total * (2 * loss_error + e ** 3 / 3 * 2 * float(slopes.abs().max()) ** 3)
+        assert abs(got - want) <= bound and abs(want) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_operands_off_their_alignment(dtype):
+    N, V, D = 70, 200, 128
+    h, w, y, dl = _operands(dtype, N, V, D, 9)
+    fh, fw = torch.zeros(N * D + 1, dtype=h.dtype, device="cuda"), torch.zeros(V * D + 1, dtype=h.dtype, device="cuda")
+    fh[1:], fw[1:] = h.reshape(-1), w.reshape(-1)
+    _reference(h, w, y, dl, dtype, *_run(fh[1:].view(N, D), fw[1:].view(V, D), y, dl, dtype))
+
+
+@pytest.mark.gpu
+def test_no_rows():
+    h, w, y, dl = _operands("bfloat16", 0, 50, 16, 10)
+    loss, lse, dh, dw = _run(h, w, y, dl, "bfloat16")
+    assert loss.shape == lse.shape == (0,) and dh.shape == (0, 16) and not dw.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_replay_from_a_graph(config, dtype):
+    N, V, D = 200, 900, 80
+    config("ce.piece_rows", 512)
+    h, w, y, dl = _operands(dtype, N, V, D, 11)
+    ph = [placeholder((N, D), dtype), placeholder((V, D), dtype), placeholder((N,), "int32")]
+    f, g = LinearCrossEntropyhip(), LinearCrossEntropyGradhip()
+    f.build(ph), g.build(ph)
+
+    def step():
+        loss, lse = f.run([h, w, y])
+        return (loss, lse) + tuple(g.run([h, w, y, lse, dl]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for k in range(3):
+        for x, new in zip((h, w, y, dl), _operands(dtype, N, V, D, 20 + k)):
+            x.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.tensor.clone() for o in out]
+        assert all(torch.equal(a, b.tensor) for a, b in zip(got, step()))
+        _reference(h, w, y, dl, dtype, *got)
+
+
+@pytest.mark.gpu
+def test_refusals():
+    ph = [placeholder((6, 8)), placeholder((10, 8)), placeholder((6,), "int32")]
+    m = LinearCrossEntropyhip()
+    h, w, y, dl = _operands("float32", 6, 10, 8, 12)
+    with pytest.raises(RuntimeError):
+        m.run([h, w, y])
+    for bad in ([placeholder((6, 8), "float16"), placeholder((10, 8), "float16"), ph[2]],
+                [ph[0], placeholder((10, 8), "bfloat16"), ph[2]], [ph[0], ph[1], placeholder((6,), "float32")]):
+        with pytest.raises(TypeError):
+            m.build(bad)
+    for bad in ([ph[0], placeholder((10, 9)), ph[2]], [ph[0], ph[1], placeholder((5,), "int32")], ph[:2],
+                [ph[0], placeholder((0, 8)), ph[2]], [placeholder((2 ** 23, 8)), ph[1], placeholder((2 ** 23,), "int32")]):
+        with pytest.raises(ValueError):
+            m.build(bad)
+    m.build(ph)
+    for bad in ([h[:5], w, y], [h, w[:9], y], [h, w], [h.cpu(), w, y], [h, w.t().contiguous().t(), y]):
+        with pytest.raises(ValueError):
+            m.run(bad)
+    for bad in ([h.bfloat16(), w, y], [h, w, y.long()]):
+        with pytest.raises(TypeError):
+            m.run(bad)
+    g = LinearCrossEntropyGradhip()
+    g.build(ph)
+    _, lse = m.run([h, w, y])
+    with pytest.raises(ValueError):
+        g.run([h, w, y, lse])
+    with pytest.raises(ValueError):
+        g.run([g._dhidden, w, y, lse, dl])                              # an output as an operand
+    with pytest.raises(TypeError):
+        g.run([h, w, y, lse.tensor.double(), dl])
+
+
+def test_bad_arguments_of_the_entry_points_without_a_device():
+    L = _lib.lib()
+    need = ctypes.c_int64(0)
+    for sizes in ((-1, 4, 4), (4, 0, 4), (4, 4, 0), (2 ** 23, 4, 4), (4, 2 ** 31, 4), (4, 4, 2 ** 17)):
+        assert L.fg_linear_ce_workspace(*sizes, 0, ctypes.byref(need)) == -1
+        assert L.fg_linear_ce(*sizes, 16, 16, 16, 16, 16, 0, 0, 256, 1 << 40, None) == -1
+        assert L.fg_linear_ce_grad(*sizes, 16, 16, 16, 16, 16, 16, 16, 0, 0, 256, 1 << 40, None) == -1
+    assert L.fg_linear_ce_workspace(4, 4, 4, 2, ctypes.byref(need)) == -4               # float16
+    assert L.fg_linear_ce_workspace(4, 4, 4, 0, None) == -1
+    assert L.fg_linear_ce_workspace(4, 4, 4, 0, ctypes.byref(need)) == 0 and need.value > 0
+    assert L.fg_linear_ce(4, 4, 4, 16, 16, 16, 16, 16, 0, 2, 256, need.value, None) == -1        # no such index type
+    assert L.fg_linear_ce(4, 4, 4, 16, None, 16, 16, 16, 0, 0, 256, need.value, None) == -1
+    assert L.fg_linear_ce(4, 4, 4, 16, 16, 16, 16, 16, 0, 0, 256, 16, None) == -1                # workspace too small
+    assert b"workspace" in L.fg_last_error()
+    assert L.fg_linear_ce(0, 4, 4, None, None, None, None, None, 0, 0, None, 0, None) == 0
+    assert L.fg_linear_ce_grad_workspace(4, 4, 4, 0, ctypes.byref(need)) == 0
+    assert L.fg_linear_ce_grad(4, 4, 4, 16, 16, 16, 16, None, 16, 16, 0, 0, 256, need.value, None) == -1
+    assert L.fg_linear_ce_grad(4, 4, 4, 16, 16, 16, 16, 16, 16, 16, 0, 0, 264, need.value, None) == -1
