@@ -2,29 +2,41 @@
 //
 //   l[n, v]  = <h[n], w[v]>                    lse[n] = log sum over v of exp l[n, v]
 //   loss[n]  = lse[n] - l[n, y[n]]             (0 where the label y[n] is outside [0, V): the row is ignored)
-//   G[n, v]  = dloss[n] * (exp(l[n, v] - lse[n]) - [v = y[n]])          (0 for an ignored row)
-//   dh = G w        dw = G^T h
+//   P[n, v]  = exp(l[n, v] - lse[n]) - [v = y[n]]          (0 for an ignored row)
+//   dh[n]    = dloss[n] * sum over v of P[n, v] w[v]       dw[v] = sum over n of P[n, v] dloss[n] h[n]
 //
 // Forward: one matrix product whose epilogue keeps, per row n and tile of vocabulary, the largest logit and the sum
 // of exponentials relative to it; a second kernel joins the tiles and takes the label's logit as a dot product of its
-// own.  Backward: the logits are computed again piece by piece of the vocabulary; the epilogue turns them into G,
+// own.  Backward: the logits are computed again piece by piece of the vocabulary; the epilogue turns them into P,
 // written once as [n, v] and once as [v, n], and two more products over them give the piece's rows of dw and its
 // share of dh.  All three products are the same kernel over operands with k contiguous, so h and w are transposed
 // into padded copies for the backward products (2 N D + 2 V D elements of traffic against 6 N V D flops).
 //
-// Types: bfloat16 operands are used as they are; G is rounded to bfloat16 for the products (half a step, 2^-9 of each
-// term, random in sign; the results are rounded to bfloat16 themselves), everything between is float32.  float32
-// operands, G among them, are split into three bfloat16 parts (mfma_gemm.hpp), which keeps float32's accuracy: six
-// bfloat16 products run at 2.6 times the peak rate of the float32 matrix instructions.
+// Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step of each
+// term, random in sign; the results are rounded to bfloat16 themselves); everything between is float32.  float32
+// operands, P among them, are split into two float16 parts (mfma_gemm.hpp), which keeps float32's accuracy.  P is at
+// most 1 and stored times 2^14; dloss is applied to the rows of dh in the epilogue and to the copy of h for dw.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "mfma_gemm.hpp"
 
 namespace fg {
 namespace {
 
+// Keeps the compiler from moving the work of one block of accumulators into another's, which costs registers.
+#if defined(__HIP_DEVICE_COMPILE__)
+#define FG_IN_ORDER() __builtin_amdgcn_sched_barrier(0)
+// ... and fixes the point at which x is computed.
+#define FG_HERE(x) asm volatile("" : "+v"(x))
+#else
+#define FG_IN_ORDER()
+#define FG_HERE(x)
+#endif
+
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kTop = 14;  // binary exponent that a scaled float32 operand's largest element is brought to
 
 using Big = GemmTile<256, 256, 2, 4>;   // 128 x 64 per wave, one workgroup per CU
 using Mid = GemmTile<128, 128, 2, 2>;   // 64 x 64 per wave, two workgroups per CU
@@ -32,89 +44,138 @@ using Flat = GemmTile<64, 256, 1, 4>;   // few rows of A
 using Tall = GemmTile<256, 64, 4, 1>;   // few rows of B
 
 // ------------------------------------------------------------------------------------------------ operand copies
-struct Split {
-  uint16_t part[kParts];
-};
-__device__ __forceinline__ uint16_t bits_of(float x) { return __builtin_bit_cast(uint16_t, narrow<__bf16>(x)); }
-__device__ __forceinline__ float from_bits(uint16_t b) { return __builtin_bit_cast(float, static_cast<uint32_t>(b) << 16); }
+__device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint16_t, narrow<__bf16>(x)); }
+__device__ __forceinline__ uint32_t half_bits(float x) { return __builtin_bit_cast(uint16_t, narrow<_Float16>(x)); }
 
-// x = part 0 + part 1 + part 2 to 2^-24 of x and better.  A finite x that would round to infinity is cut instead; what is
-// not finite has no further parts, so that it does not turn into NaN by inf - inf.
-__device__ __forceinline__ Split split3(float x) {
-  Split s;
-  uint32_t u = __builtin_bit_cast(uint32_t, x);
-  s.part[0] = bits_of(x);
-  if ((s.part[0] & 0x7f80) == 0x7f80) {
-    if ((u & 0x7f800000u) == 0x7f800000u) {
-      s.part[1] = s.part[2] = 0;
-      return s;
-    }
-    s.part[0] = static_cast<uint16_t>(u >> 16);
-  }
-  const float r = x - from_bits(s.part[0]);
-  s.part[1] = bits_of(r);
-  s.part[2] = bits_of(r - from_bits(s.part[1]));
-  return s;
-}
-
+// Part `part` of x, whose exponent has been brought into float16's range.  What is not finite has no second part, so
+// that it does not turn into NaN by inf - inf.
 template <typename T>
-__device__ __forceinline__ void store_parts(uint16_t *out, int64_t at, int64_t part, float x) {
-  if constexpr (sizeof(T) == 4) {
-    const Split s = split3(x);
-#pragma unroll
-    for (int p = 0; p < kParts; ++p) out[p * part + at] = s.part[p];
+__device__ __forceinline__ uint32_t part_of(float x, int part) {
+  if constexpr (sizeof(T) == 2) {
+    return bits_of(x);
   } else {
-    out[at] = bits_of(x);
+    const _Float16 hi = narrow<_Float16>(x);
+    if (part == 0) return __builtin_bit_cast(uint16_t, hi);
+    const float rest = x - widen(hi);
+    return half_bits(__builtin_fabsf(x) < INFINITY ? rest * (1 << kLowBits) : 0.0f);
   }
 }
 
-// [rows, D] -> parts of [rows, Dp], zeros behind D
-template <typename T>
-__global__ __launch_bounds__(kBlockThreads) void pack_kernel(const T *x, uint16_t *out, int64_t rows, int32_t D,
-                                                             int32_t Dp) {
+// The exponent that brings a largest element (as float bits) to 2^kTop; 0 when there is none.
+__device__ __forceinline__ int exponent_for(uint32_t peak) {
+  if (peak == 0) return 0;
+  return min(126, max(-126, kTop - (static_cast<int>(peak >> 23) - 127)));
+}
+
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+
+// bfloat16: [rows, D] -> [rows, Dp], zeros behind D
+__global__ __launch_bounds__(kBlockThreads) void pad_kernel(const uint16_t *x, uint16_t *out, int64_t rows, int32_t D,
+                                                            int32_t Dp) {
   const int64_t total = rows * Dp, stride = static_cast<int64_t>(gridDim.x) * kBlockThreads;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x; t < total; t += stride) {
     const int64_t r = t / Dp;
     const int32_t c = static_cast<int32_t>(t - r * Dp);
-    store_parts<T>(out, t, total, c < D ? widen(x[r * D + c]) : 0.0f);
+    out[t] = c < D ? x[r * D + c] : 0;
   }
 }
 
-// [rows, D] -> parts of [D, pitch], zeros behind the rows and, with `keep`, in place of rows whose keep[] is negative
-// (whatever those hold must not reach the sum over rows)
-template <typename T>
-__global__ __launch_bounds__(kBlockThreads) void transpose_kernel(const T *x, const int32_t *keep, uint16_t *out,
-                                                                  int32_t rows, int32_t D, int64_t pitch) {
+// float32: [rows, D] -> two parts of [rows, Dp], zeros behind D, each row by its own exponent (exps).  One wave per row.
+// peak (or null): largest |x| * |factor[row]| over the rows whose keep[] is not negative, for the transposed copy.
+__global__ __launch_bounds__(kBlockThreads) void split_rows_kernel(const float *x, uint16_t *out, int64_t rows,
+                                                                   int32_t D, int32_t Dp, int32_t *exps, uint32_t *peak,
+                                                                   const int32_t *keep, const float *factor) {
+  __shared__ uint32_t peaks[kWavesPerBlock];
+  const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
+  const int64_t part = rows * Dp, stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
+  uint32_t most = 0;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave; r < rows; r += stride) {
+    const float *row = x + r * D;
+    uint32_t top = 0;
+    for (int32_t c = lane; c < D; c += kWaveSize) top = max(top, finite_bits(row[c]));
+#pragma unroll
+    for (int d = 1; d < kWaveSize; d <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, kWaveSize)));
+    const int e = exponent_for(top);
+    if (lane == 0) exps[r] = e;
+    for (int32_t c = lane; c < Dp; c += kWaveSize) {
+      const float y = c < D ? __builtin_ldexpf(row[c], e) : 0.0f;
+      out[r * Dp + c] = static_cast<uint16_t>(part_of<float>(y, 0));
+      out[part + r * Dp + c] = static_cast<uint16_t>(part_of<float>(y, 1));
+    }
+    if (peak && (!keep || keep[r] >= 0))
+      most = max(most, finite_bits(__builtin_bit_cast(float, top) * (factor ? factor[r] : 1.0f)));
+  }
+  if (!peak) return;
+  if (lane == 0) peaks[wave] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kWavesPerBlock; ++w) most = max(most, peaks[w]);
+    atomicMax(peak, most);  // a largest value does not depend on the order
+  }
+}
+
+// [rows, D] -> parts of [D, pitch], zeros behind the rows and in place of rows whose keep[] is negative (whatever those
+// hold must not reach the sum over rows).  float32: times factor[row] (or 1) and brought into range by *peak.
+// 64 x 64 elements per workgroup, 16 bytes per lane on both sides where D allows (kVec elements per load).
+template <typename T, int kVec>
+__global__ __launch_bounds__(kBlockThreads) void transpose_kernel(const T *x, const int32_t *keep, const float *factor,
+                                                                  const uint32_t *peak, uint16_t *out, int32_t rows,
+                                                                  int32_t D, int64_t pitch) {
+  constexpr int kLanes = 64 / kVec;  // per row
   __shared__ float tile[64][65];
-  const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64;
-  const int low = threadIdx.x & 63, high = threadIdx.x >> 6;
-  for (int k = high; k < 64; k += kWavesPerBlock) {
-    const int r = r0 + k, c = c0 + low;
-    float v = 0.0f;
-    if (r < rows && c < D && (!keep || keep[r] >= 0)) v = widen(x[static_cast<int64_t>(r) * D + c]);
-    tile[k][low] = v;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
+  const int c0 = blockIdx.y * 64;
+  const int e = peak ? exponent_for(*peak) : 0;
+  const int c = c0 + threadIdx.x % kLanes * kVec;
+  for (int k = threadIdx.x / kLanes; k < 64; k += kBlockThreads / kLanes) {
+    const int64_t r = r0 + k;
+    Pack<T, kVec> v;
+    const bool there = r < rows && c < D && (!keep || keep[r] >= 0);
+    if (there) v = *reinterpret_cast<const Pack<T, kVec> *>(x + r * D + c);
+    const float f = sizeof(T) == 4 && there && factor ? factor[r] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      float y = there ? widen(v.v[j]) : 0.0f;
+      if constexpr (sizeof(T) == 4) y = there ? __builtin_ldexpf(y * f, e) : 0.0f;
+      tile[k][threadIdx.x % kLanes * kVec + j] = y;
+    }
   }
   __syncthreads();
-  for (int k = high; k < 64; k += kWavesPerBlock) {
-    const int r = r0 + low, c = c0 + k;
-    if (c < D && r < pitch) store_parts<T>(out, static_cast<int64_t>(c) * pitch + r, D * pitch, tile[low][k]);
+  for (int t = threadIdx.x; t < 512; t += kBlockThreads) {  // eight rows of one column each
+    const int g = t % 8, col = t / 8;
+    const int64_t r = r0 + 8 * g;
+    if (c0 + col >= D || r >= pitch) continue;
+#pragma unroll
+    for (int p = 0; p < Multiply<T>::kParts; ++p) {
+      Pack<uint16_t, 8> y;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y.v[k] = static_cast<uint16_t>(part_of<T>(tile[8 * g + k][col], p));
+      *reinterpret_cast<Pack<uint16_t, 8> *>(out + p * D * pitch + static_cast<int64_t>(c0 + col) * pitch + r) = y;
+    }
   }
 }
 
+// Labels as int32, -1 for rows to ignore; clears the words that collect the largest elements.
 template <typename Id>
-__global__ __launch_bounds__(kBlockThreads) void labels_kernel(const Id *labels, int32_t n, int64_t V, int32_t *out) {
+__global__ __launch_bounds__(kBlockThreads) void labels_kernel(const Id *labels, int32_t n, int64_t V, int32_t *out,
+                                                               uint32_t *peaks, int32_t n_peaks) {
   const int i = blockIdx.x * kBlockThreads + threadIdx.x;
   if (i < n) {
     const Id y = labels[i];
     out[i] = y >= 0 && static_cast<int64_t>(y) < V ? static_cast<int32_t>(y) : -1;
   }
+  for (int k = i; k < n_peaks; k += gridDim.x * kBlockThreads) peaks[k] = 0;
 }
 
 // ------------------------------------------------------------------------------------------------ forward
 struct StatsArgs {
-  GemmShape g;
-  float2 *part;      // [tiles of vocabulary, N]: largest logit, sum of exp(l - largest)
-  int32_t tile0;     // first tile of this piece
+  GemmShape g;             // a: rows of w, b: h
+  const int32_t *exp_a, *exp_b;  // float32: exponents of the rows
+  float2 *part;            // [tiles of vocabulary, N]: largest logit, sum of exp(l - largest)
+  int32_t tile0;           // first tile of this piece
 };
 
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
@@ -123,16 +184,50 @@ __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
   return float2{m, a.y * __builtin_amdgcn_exp2f((a.x - m) * kLog2e) + b.y * __builtin_amdgcn_exp2f((b.x - m) * kLog2e)};
 }
 
-template <typename Tile>
+// Takes the rows' exponents back out of the accumulators: what is left are the logits.
+template <typename Tile, typename T>
+__device__ __forceinline__ void to_logits(GemmAcc<Tile> &acc, const int32_t *exp_a, const int32_t *exp_b, int64_t v0,
+                                          int64_t n0, int32_t N, int lane) {
+  if constexpr (sizeof(T) == 4) {
+    int en[Tile::TN];
+#pragma unroll
+    for (int j = 0; j < Tile::TN; ++j) {
+      const int64_t n = n0 + 32 * j + lane % 32;
+      en[j] = n < N ? exp_b[n] : 0;
+    }
+#pragma unroll
+    for (int i = 0; i < Tile::TM; ++i) {
+      FG_IN_ORDER();
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int4 ev = *reinterpret_cast<const int4 *>(exp_a + v0 + 32 * i + acc_row(4 * q, lane));
+#pragma unroll
+        for (int j = 0; j < Tile::TN; ++j) {
+          const int en_ev[4] = {en[j] + ev.x, en[j] + ev.y, en[j] + ev.z, en[j] + ev.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float x = __builtin_ldexpf(acc.c[i][j][4 * q + k], -en_ev[k]);
+            FG_HERE(x);  // done here, so that the exponents' registers are free again
+            acc.c[i][j][4 * q + k] = x;
+          }
+        }
+      }
+    }
+  }
+}
+
+template <typename Tile, typename T>
 __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
   const GemmPlace at = gemm_place(a.g);
-  gemm_tile<Tile>(a.g, at, lds, acc);
+  gemm_tile<Tile, T>(a.g, at, lds, acc);
   __syncthreads();
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
   const int v0 = at.tm * Tile::BM + wm * (Tile::BM / Tile::WM);
+  const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wn * (Tile::BN / Tile::WN);
+  to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
   float2 *stats = reinterpret_cast<float2 *>(lds);  // [WM][BN]
   const bool edge = v0 + Tile::BM / Tile::WM > a.g.a.rows;
 #pragma unroll
@@ -170,111 +265,162 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   }
 }
 
-// 64 rows per workgroup: its 16 waves share the tiles of vocabulary, then take four rows' labels each.
-constexpr int kLossThreads = 1024;
-template <typename T, typename Id>
-__global__ __launch_bounds__(kLossThreads) void loss_kernel(const float2 *part, int32_t tiles, const T *h, const T *w,
-                                                            const Id *labels, int32_t N, int64_t V, int32_t D,
-                                                            float *loss, float *lse) {
-  constexpr int kWaves = kLossThreads / kWaveSize;
-  __shared__ float2 joined[kWaves][kWaveSize];
-  __shared__ float row_lse[kWaveSize];
-  const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * kWaveSize + lane;
+// 16 rows per workgroup.  Its threads, 16 neighbouring ones per tile, share the tiles of vocabulary; then its waves take
+// the rows' labels, kVec elements per lane and step of the dot product.
+constexpr int kLossRows = 16;
+template <typename T, typename Id, int kVec, int kThreads>
+__global__ __launch_bounds__(kThreads) void loss_kernel(const float2 *part, int32_t tiles, const T *h, const T *w,
+                                                        const Id *labels, int32_t N, int64_t V, int32_t D, float *loss,
+                                                        float *lse) {
+  constexpr int kShares = kThreads / kLossRows, kWaves = kThreads / kWaveSize;
+  __shared__ float2 joined[kShares][kLossRows];
+  __shared__ float row_lse[kLossRows];
+  const int row = threadIdx.x % kLossRows, share = threadIdx.x / kLossRows;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kLossRows;
   float2 s{-INFINITY, 0.0f};
-  if (n < N)
-    for (int32_t t = wave; t < tiles; t += kWaves) s = join_stats(s, part[static_cast<int64_t>(t) * N + n]);
-  joined[wave][lane] = s;
-  __syncthreads();
-  if (wave == 0) {
-#pragma unroll
-    for (int k = 1; k < kWaves; ++k) s = join_stats(s, joined[k][lane]);
+  if (n0 + row < N)
+    for (int32_t t = share; t < tiles; t += kShares) s = join_stats(s, part[static_cast<int64_t>(t) * N + n0 + row]);
+  joined[share][row] = s;
+  for (int half = kShares / 2; half > 0; half >>= 1) {
+    __syncthreads();
+    if (share < half) joined[share][row] = s = join_stats(s, joined[share + half][row]);
+  }
+  if (share == 0) {
     const float r = s.x + logf(s.y);
-    row_lse[lane] = r;
-    if (n < N) lse[n] = r;
+    row_lse[row] = r;
+    if (n0 + row < N) lse[n0 + row] = r;
   }
   __syncthreads();
-  for (int k = wave; k < kWaveSize; k += kWaves) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kWaveSize + k;
-    if (i >= N) break;
-    const Id y = labels[i];
+  const int lane = threadIdx.x & (kWaveSize - 1);
+  for (int k = threadIdx.x / kWaveSize; k < kLossRows && n0 + k < N; k += kWaves) {
+    const Id y = labels[n0 + k];
     const bool there = y >= 0 && static_cast<int64_t>(y) < V;
     float dot = 0.0f;
     if (there) {
-      const T *a = h + i * D, *b = w + static_cast<int64_t>(y) * D;
-      for (int32_t c = lane; c < D; c += kWaveSize) dot = __builtin_fmaf(widen(a[c]), widen(b[c]), dot);
+      using P = Pack<T, kVec>;
+      const T *a = h + (n0 + k) * D, *b = w + static_cast<int64_t>(y) * D;
+      for (int32_t c = lane * kVec; c < D; c += kWaveSize * kVec) {
+        const P pa = *reinterpret_cast<const P *>(a + c), pb = *reinterpret_cast<const P *>(b + c);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) dot = __builtin_fmaf(widen(pa.v[j]), widen(pb.v[j]), dot);
+      }
 #pragma unroll
       for (int d = 1; d < kWaveSize; d <<= 1) dot += __shfl_xor(dot, d, kWaveSize);
     }
-    if (lane == 0) loss[i] = there ? row_lse[k] - dot : 0.0f;
+    if (lane == 0) loss[n0 + k] = there ? row_lse[k] - dot : 0.0f;
   }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
+// Four lanes that hold the same four rows of four neighbouring columns, two 16-bit elements per word (rows 0, 1 in a,
+// rows 2, 3 in b), turn them: afterwards lane q of the four holds row q, its four columns in a (0, 1) and b (2, 3).
+__device__ __forceinline__ uint2 turn4(uint2 x, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E;  // quad permutations: lane ^ 1, lane ^ 2
+  const uint32_t ta = __builtin_amdgcn_mov_dpp(x.x, kSwap1, 0xf, 0xf, true);
+  const uint32_t tb = __builtin_amdgcn_mov_dpp(x.y, kSwap1, 0xf, 0xf, true);
+  const uint32_t pick = lane & 1 ? 0x03020706u : 0x05040100u;  // even: own and other's low half; odd: the high halves
+  const uint32_t a = __builtin_amdgcn_perm(ta, x.x, pick), b = __builtin_amdgcn_perm(tb, x.y, pick);
+  const uint32_t got = __builtin_amdgcn_mov_dpp(lane & 2 ? a : b, kSwap2, 0xf, 0xf, true);
+  return lane & 2 ? uint2{got, b} : uint2{a, got};
+#else
+  return x;
+#endif
+}
+
 struct GradArgs {
   GemmShape g;               // a: the piece's rows of w, b: h
+  const int32_t *exp_a, *exp_b;
   const int32_t *label;      // [N], negative: ignored
   const float *lse, *dloss;  // [N]
   int32_t v0;                // first vocabulary row of the piece
-  uint16_t *nv, *vn;         // G as [N, pitch_v] and [rows of the piece, pitch_n], parts apart by *_part
+  uint16_t *nv, *vn;         // P as [N, pitch_v] and [rows of the piece, pitch_n], parts apart by *_part
   int64_t nv_part, vn_part;
-  int32_t pitch_v, pitch_n;
+  int32_t pitch_v, pitch_n;  // multiples of 64; what is behind the ends is written as zeros
 };
 
-// T: type of the operands, which says how G is stored.
+// T: type of the operands, which says how P is stored.  The [v, n] copy is written from the registers, four n per lane;
+// the [n, v] copy goes through LDS, so that its rows leave in 16-byte pieces that follow each other (a 16-byte piece of
+// row n lies at piece ^ n within the row, so that neither side meets bank conflicts).
 template <typename Tile, typename T>
 __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
   const GemmPlace at = gemm_place(a.g);
-  gemm_tile<Tile>(a.g, at, lds, acc);
+  gemm_tile<Tile, T>(a.g, at, lds, acc);
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
-  const int v0 = at.tm * Tile::BM + wm * (Tile::BM / Tile::WM);
-  const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wn * (Tile::BN / Tile::WN);
+  const int wave_v = wm * (Tile::BM / Tile::WM), wave_n = wn * (Tile::BN / Tile::WN);
+  const int v0 = at.tm * Tile::BM + wave_v;
+  const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wave_n;
+  to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
+  const bool edge = v0 + Tile::BM / Tile::WM > a.g.a.rows;
 #pragma unroll
   for (int j = 0; j < Tile::TN; ++j) {
     const int64_t n = n0 + 32 * j + lane % 32;
-    const bool row = n < a.g.b.rows;
-    const int32_t label = row ? a.label[n] : -1;
-    const float lse = row ? a.lse[n] : 0.0f, dl = label >= 0 ? a.dloss[n] : 0.0f;
+    const int32_t label = n < a.g.b.rows ? a.label[n] : -1;
+    const float lse = label >= 0 ? a.lse[n] : 0.0f;
+    const float times = sizeof(T) == 4 ? static_cast<float>(1 << kTop) : label >= 0 ? a.dloss[n] : 0.0f;
     const int32_t hit = label >= 0 ? label - a.v0 - v0 : -1;  // row of this wave's block that is the label's
     const bool any_hit = __any(hit >= 0 && hit < Tile::BM / Tile::WM);
 #pragma unroll
     for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float x[4];
+      for (int r = 0; r < 16; ++r) {
+        const int v = 32 * i + acc_row(r, lane);
+        float p = __builtin_amdgcn_exp2f((acc.c[i][j][r] - lse) * kLog2e);
+        if (any_hit && v == hit) p -= 1.0f;
+        acc.c[i][j][r] = label >= 0 && !(edge && v0 + v >= a.g.a.rows) ? p * times : 0.0f;
+      }
+  }
+  constexpr int kPieces = Tile::BM / 8;  // of 16 bytes in a row of the [n, v] tile
+  auto place = [](int n, int piece) { return piece ^ (kPieces == 8 ? (n >> 1) & 7 : n & (kPieces - 1)); };
+  // the 16-bit form of the accumulator x; a float32's rest takes its place for the next part
+  auto take = [](float &x) -> uint32_t {
+    const uint32_t bits = part_of<T>(x, 0);
+    if constexpr (sizeof(T) == 4) {
+      x = (x - widen(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)))) * (1 << kLowBits);
+      FG_HERE(x);  // in x's place, not beside it
+    }
+    return bits;
+  };
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = 4 * q + k, v = 32 * i + acc_row(r, lane);
-          float p = __builtin_amdgcn_exp2f((acc.c[i][j][r] - lse) * kLog2e);
-          if (any_hit && v == hit) p -= 1.0f;
-          x[k] = label >= 0 && v0 + v < a.g.a.rows ? p * dl : 0.0f;
-          if (v0 + v < a.g.a.rows && n < a.pitch_n)
-            store_parts<T>(a.vn, static_cast<int64_t>(v0 + v) * a.pitch_n + n, a.vn_part, x[k]);
-        }
-        const int v = v0 + 32 * i + acc_row(4 * q, lane);
-        if (row && v < a.pitch_v) {
-          uint16_t *to = a.nv + n * a.pitch_v + v;
-          if constexpr (sizeof(T) == 4) {
-            Pack<uint16_t, 4> y[kParts];
+  for (int part = 0; part < Multiply<T>::kParts; ++part) {
+    __syncthreads();  // the operands, or the first part, are no longer read
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const Split s = split3(x[k]);
+    for (int j = 0; j < Tile::TN; ++j)
 #pragma unroll
-              for (int p = 0; p < kParts; ++p) y[p].v[k] = s.part[p];
-            }
+      for (int i = 0; i < Tile::TM; ++i) {
+        FG_IN_ORDER();
 #pragma unroll
-            for (int p = 0; p < kParts; ++p) *reinterpret_cast<Pack<uint16_t, 4> *>(to + p * a.nv_part) = y[p];
-          } else {
-            Pack<uint16_t, 4> y;
+        for (int q = 0; q < 4; ++q) {
+          uint2 x;
+          float e[4] = {acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
+          x.x = take(e[0]);
+          x.x |= take(e[1]) << 16;
+          x.y = take(e[2]);
+          x.y |= take(e[3]) << 16;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) y.v[k] = bits_of(x[k]);
-            *reinterpret_cast<Pack<uint16_t, 4> *>(to) = y;
-          }
+          for (int k = 0; k < 4; ++k) acc.c[i][j][4 * q + k] = e[k];
+          const int n = wave_n + 32 * j + lane % 32, v = wave_v + 32 * i + 8 * q;  // lanes 32..63: the second half
+          *reinterpret_cast<uint2 *>(lds + n * Tile::BM + place(n, v / 8) * 8 + lane / 32 * 4) = x;
+          const uint2 y = turn4(x, lane);
+          const int row = v0 + 32 * i + acc_row(4 * q, lane) + lane % 4;
+          const int64_t col = n0 + 32 * j + lane % 32 / 4 * 4;
+          if (row < a.g.a.rows && col < a.pitch_n)
+            *reinterpret_cast<uint2 *>(a.vn + part * a.vn_part + static_cast<int64_t>(row) * a.pitch_n + col) = y;
         }
       }
+    __syncthreads();
+    const int64_t first_n = static_cast<int64_t>(at.tn) * Tile::BN;
+    const int first_v = at.tm * Tile::BM;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < Tile::BN * kPieces; t += Tile::kThreads) {
+      const int n = t / kPieces, piece = t % kPieces;
+      if (first_n + n < a.g.b.rows && first_v + piece * 8 < a.pitch_v)
+        *reinterpret_cast<uint4 *>(a.nv + part * a.nv_part + (first_n + n) * a.pitch_v + first_v + piece * 8) =
+            *reinterpret_cast<const uint4 *>(lds + n * Tile::BM + place(n, piece) * 8);
+    }
   }
 }
 
@@ -282,9 +428,12 @@ struct StoreArgs {
   GemmShape g;
   void *out;               // [rows of a, rows of b] of T
   const int32_t *keep;     // rows of a to write as zeros where negative (null: none)
+  const float *factor;     // float32: of the rows of a (null: 1)
+  const uint32_t *peak;    // float32: what operand b was scaled by; a is P times 2^kTop
   float *part;             // or float32 sums of each split, [splits, part_stride], added to what is there
   int64_t part_stride;
   int32_t accumulate;
+  int32_t wide;            // 16-bit out: four elements per store (its alignment and the row length allow it)
 };
 
 // kPartial: the sums go to a.part for join_kernel, else rounded to a.out.
@@ -293,28 +442,54 @@ __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
   const GemmPlace at = gemm_place(a.g);
-  gemm_tile<Tile>(a.g, at, lds, acc);
+  gemm_tile<Tile, T>(a.g, at, lds, acc);
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
   const int64_t m0 = static_cast<int64_t>(at.tm) * Tile::BM + wm * (Tile::BM / Tile::WM);
   const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wn * (Tile::BN / Tile::WN);
+  const int64_t M = a.g.a.rows, N = a.g.b.rows;
+  if constexpr (sizeof(T) == 2 && !kPartial) {
+    if (a.wide) {
+#pragma unroll
+      for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int64_t m = m0 + 32 * i + acc_row(4 * q, lane) + lane % 4;
+          const bool zero = m < M && a.keep && a.keep[m] < 0;
+#pragma unroll
+          for (int j = 0; j < Tile::TN; ++j) {
+            uint2 x;
+            x.x = bits_of(acc.c[i][j][4 * q]) | bits_of(acc.c[i][j][4 * q + 1]) << 16;
+            x.y = bits_of(acc.c[i][j][4 * q + 2]) | bits_of(acc.c[i][j][4 * q + 3]) << 16;
+            x = turn4(x, lane);
+            const int64_t n = n0 + 32 * j + lane % 32 / 4 * 4;
+            if (m < M && n < N) *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + m * N + n) = zero ? uint2{0, 0} : x;
+          }
+        }
+      return;
+    }
+  }
+  const int e = sizeof(T) == 4 ? -(kTop + exponent_for(*a.peak)) : 0;
   float *part = kPartial ? a.part + at.split * a.part_stride : nullptr;
 #pragma unroll
   for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int64_t m = m0 + 32 * i + acc_row(r, lane);
-      if (m >= a.g.a.rows) continue;
+      if (m >= M) continue;
       const bool zero = !kPartial && a.keep && a.keep[m] < 0;
+      const float f = sizeof(T) == 4 && a.factor ? a.factor[m] : 1.0f;
 #pragma unroll
       for (int j = 0; j < Tile::TN; ++j) {
         const int64_t n = n0 + 32 * j + lane % 32;
-        if (n >= a.g.b.rows) continue;
-        const int64_t to = m * a.g.b.rows + n;
+        if (n >= N) continue;
+        const int64_t to = m * N + n;
+        float x = acc.c[i][j][r];
+        if constexpr (sizeof(T) == 4) x = __builtin_ldexpf(x, e) * f;
         if constexpr (kPartial)
-          part[to] = a.accumulate ? part[to] + acc.c[i][j][r] : acc.c[i][j][r];
+          part[to] = a.accumulate ? part[to] + x : x;
         else
-          static_cast<T *>(a.out)[to] = narrow<T>(zero ? 0.0f : acc.c[i][j][r]);
+          static_cast<T *>(a.out)[to] = narrow<T>(zero ? 0.0f : x);
       }
     }
 }
@@ -379,26 +554,29 @@ constexpr int64_t kPieceBytes = int64_t{512} << 20;  // copies and G of one piec
 
 struct Layout {
   int parts, segments;
-  bool packed;           // operands copied with k padded (float32, or rows that are no multiple of 64 or 16 bytes)
+  int64_t pieces;
+  bool packed;           // operands copied with k padded (float32, or rows that are no multiple of kPadK or 16 bytes)
   int64_t Dp, Np;        // D and N to multiples of 64
   int64_t piece;         // vocabulary rows per piece, a multiple of 256
   TileKind logits, dh, dw;
   int dh_splits, dw_splits;
-  int64_t h_pack, w_pack, stats, label, ht, wt, nv, vn, dh_part, dw_part, bytes;
+  int64_t h_pack, w_pack, h_exp, w_exp, peaks, stats, label, ht, wt, nv, vn, dh_part, dw_part, bytes;
 };
 
 Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool backward) {
   Layout l{};
   l.parts = dtype == FG_F32 ? kParts : 1;
   l.segments = dtype == FG_F32 ? kSegments : 1;
-  l.packed = dtype == FG_F32 || D % kStepK != 0 || !aligned;
-  l.Dp = up(D, kStepK);
-  l.Np = up(N, kStepK);
+  l.packed = dtype == FG_F32 || D % kPadK != 0 || !aligned;
+  l.Dp = up(D, kPadK);
+  l.Np = up(N, kPadK);
   int64_t per_row = l.packed ? 2 * l.parts * l.Dp : 0;
   if (backward) per_row += 2 * l.parts * (2 * l.Np + D);
-  l.piece = per_row ? std::max<int64_t>(256, std::min(up(V, 256), kPieceBytes / per_row / 256 * 256)) : up(V, 256);
+  const int64_t most = per_row ? std::max<int64_t>(256, kPieceBytes / per_row / 256 * 256) : up(V, 256);
+  l.piece = up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), 256);  // as many pieces as needed, of equal size
   if (const int64_t rows = config().ce_piece_rows) l.piece = up(rows, 256);
-  const int64_t in_piece = std::min(l.piece, V), piece_p = up(in_piece, kStepK);
+  const int64_t in_piece = std::min(l.piece, V), piece_p = up(in_piece, kPadK);
+  l.pieces = (V + l.piece - 1) / l.piece;
   l.logits = choose_tile(in_piece, N, false);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -408,9 +586,14 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   };
   l.h_pack = take(l.packed ? 2 * l.parts * N * l.Dp : 0);
   l.w_pack = take(l.packed ? 2 * l.parts * in_piece * l.Dp : 0);
+  if (dtype == FG_F32) {
+    l.h_exp = take(4 * up(N, 256));
+    l.w_exp = take(4 * up(in_piece, 256));
+    l.peaks = take(4 * (1 + l.pieces));
+  }
   if (!backward) {
     const int64_t bm = kTileSize[l.logits].bm;
-    l.stats = take(((V + l.piece - 1) / l.piece) * ((l.piece + bm - 1) / bm) * N * 8);
+    l.stats = take(l.pieces * ((l.piece + bm - 1) / bm) * N * 8);
   } else {
     l.dh = choose_tile(N, D, true);
     l.dw = choose_tile(in_piece, D, true);
@@ -450,28 +633,42 @@ unsigned flat_grid(int64_t threads) {
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((threads + kBlockThreads - 1) / kBlockThreads, 1 << 14)));
 }
 
+// x as an operand of the logits; float32 also leaves its rows' exponents and, with `peak`, its largest element.
 template <typename T>
-GemmOperand operand(const T *x, int64_t rows, int64_t D, const Layout &l, uint16_t *copy, hipStream_t stream) {
+GemmOperand operand(const T *x, int64_t rows, int64_t D, const Layout &l, char *copy, int32_t *exps, uint32_t *peak,
+                    const int32_t *keep, const float *factor, hipStream_t stream) {
   GemmOperand o;
   o.rows = static_cast<int32_t>(rows);
-  if (l.packed) {
-    pack_kernel<T><<<dim3(flat_grid(rows * l.Dp)), dim3(kBlockThreads), 0, stream>>>(x, copy, rows, static_cast<int32_t>(D),
-                                                                                    static_cast<int32_t>(l.Dp));
-    o.p = copy;
-    o.part = rows * l.Dp;
-    o.pitch = l.Dp;
-  } else {
+  if (!l.packed) {
     o.p = reinterpret_cast<const uint16_t *>(x);
     o.pitch = D;
+    return o;
   }
+  auto *to = reinterpret_cast<uint16_t *>(copy);
+  if constexpr (sizeof(T) == 4)
+    split_rows_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>((rows + kWavesPerBlock - 1) / kWavesPerBlock, 4096))),
+                        dim3(kBlockThreads), 0, stream>>>(x, to, rows, static_cast<int32_t>(D),
+                                                          static_cast<int32_t>(l.Dp), exps, peak, keep, factor);
+  else
+    pad_kernel<<<dim3(flat_grid(rows * l.Dp)), dim3(kBlockThreads), 0, stream>>>(
+        reinterpret_cast<const uint16_t *>(x), to, rows, static_cast<int32_t>(D), static_cast<int32_t>(l.Dp));
+  o.p = to;
+  o.part = rows * l.Dp;
+  o.pitch = l.Dp;
   return o;
 }
 
 template <typename T>
-void transpose(const T *x, const int32_t *keep, uint16_t *out, int64_t rows, int64_t D, int64_t pitch, hipStream_t stream) {
-  transpose_kernel<T><<<dim3(static_cast<unsigned>((pitch + 63) / 64), static_cast<unsigned>((D + 63) / 64)),
-                        dim3(kBlockThreads), 0, stream>>>(x, keep, out, static_cast<int32_t>(rows),
-                                                          static_cast<int32_t>(D), pitch);
+void transpose(const T *x, const int32_t *keep, const float *factor, const uint32_t *peak, uint16_t *out, int64_t rows,
+               int64_t D, int64_t pitch, hipStream_t stream) {
+  constexpr int kVec = 16 / sizeof(T);
+  const dim3 grid(static_cast<unsigned>((pitch + 63) / 64), static_cast<unsigned>((D + 63) / 64));
+  if (D % kVec == 0 && aligned_to(x, 16))
+    transpose_kernel<T, kVec><<<grid, dim3(kBlockThreads), 0, stream>>>(x, keep, factor, peak, out, static_cast<int32_t>(rows),
+                                                                        static_cast<int32_t>(D), pitch);
+  else
+    transpose_kernel<T, 1><<<grid, dim3(kBlockThreads), 0, stream>>>(x, keep, factor, peak, out, static_cast<int32_t>(rows),
+                                                                     static_cast<int32_t>(D), pitch);
 }
 
 template <typename T, typename Id>
@@ -480,19 +677,31 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
   StatsArgs a{};
   a.part = reinterpret_cast<float2 *>(ws + l.stats);
   a.g.steps = static_cast<int32_t>(l.Dp / kStepK);
-  a.g.segments = l.segments;
-  a.g.b = operand(h, N, D, l, reinterpret_cast<uint16_t *>(ws + l.h_pack), stream);
+  auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
+  a.exp_a = w_exp;
+  a.exp_b = h_exp;
+  a.g.b = operand(h, N, D, l, ws + l.h_pack, h_exp, nullptr, nullptr, nullptr, stream);
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
-    a.g.a = operand(w + v0 * D, std::min(l.piece, V - v0), D, l, reinterpret_cast<uint16_t *>(ws + l.w_pack), stream);
+    a.g.a = operand(w + v0 * D, std::min(l.piece, V - v0), D, l, ws + l.w_pack, w_exp, nullptr, nullptr, nullptr, stream);
     const int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3 grid) {
       using Tile = decltype(tile);
-      stats_kernel<Tile><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
+      stats_kernel<Tile, T><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
     a.tile0 += a.g.tiles_m;
   }
-  loss_kernel<T, Id><<<dim3(static_cast<unsigned>((N + kWaveSize - 1) / kWaveSize)), dim3(kLossThreads), 0, stream>>>(
-      a.part, a.tile0, h, w, labels, static_cast<int32_t>(N), V, static_cast<int32_t>(D), loss, lse);
+  const dim3 grid(static_cast<unsigned>((N + kLossRows - 1) / kLossRows));
+  auto join = [&](auto vec, auto threads) {
+    loss_kernel<T, Id, decltype(vec)::value, decltype(threads)::value><<<grid, dim3(threads.value), 0, stream>>>(
+        a.part, a.tile0, h, w, labels, static_cast<int32_t>(N), V, static_cast<int32_t>(D), loss, lse);
+  };
+  const bool wide = vector_elements(D, sizeof(T), {h, w}) >= 4;
+  using One = std::integral_constant<int, 1>;
+  using Four = std::integral_constant<int, 4>;
+  using Few = std::integral_constant<int, 256>;
+  using Many = std::integral_constant<int, 1024>;
+  if (a.tile0 > 64) wide ? join(Four{}, Many{}) : join(One{}, Many{});  // 64 threads per row, else 16
+  else wide ? join(Four{}, Few{}) : join(One{}, Few{});
   FG_HIP_TRY(hipGetLastError());
   return FG_OK;
 }
@@ -501,6 +710,7 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
 template <typename T>
 int product(TileKind kind, StoreArgs a, T *out, bool partial, hipStream_t stream) {
   a.out = out;
+  a.wide = a.g.b.rows % 4 == 0 && aligned_to(out, 8);
   return with_tile(kind, &a.g, [&](auto tile, dim3 grid) {
     using Tile = decltype(tile);
     if (partial)
@@ -524,30 +734,35 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   a.vn = vn;
   a.pitch_n = static_cast<int32_t>(l.Np);
   a.g.steps = static_cast<int32_t>(l.Dp / kStepK);
-  a.g.segments = l.segments;
-  a.g.b = operand(h, N, D, l, reinterpret_cast<uint16_t *>(ws + l.h_pack), stream);
-  transpose(h, label, ht, N, D, l.Np, stream);
+  auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
+  uint32_t *peaks = sizeof(T) == 4 ? reinterpret_cast<uint32_t *>(ws + l.peaks) : nullptr;  // of h, then of each piece of w
+  const float *factor = sizeof(T) == 4 ? dloss : nullptr;
+  a.exp_a = w_exp;
+  a.exp_b = h_exp;
+  a.g.b = operand(h, N, D, l, ws + l.h_pack, h_exp, peaks, label, factor, stream);
+  transpose(h, label, factor, peaks, ht, N, D, l.Np, stream);
   const bool dh_partial = l.dh_splits > 1 || V > l.piece;
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
-    const int64_t rows = std::min(l.piece, V - v0), rows_p = up(rows, kStepK);
+    const int64_t rows = std::min(l.piece, V - v0), rows_p = up(rows, kPadK);
     a.v0 = static_cast<int32_t>(v0);
     a.pitch_v = static_cast<int32_t>(rows_p);
     a.nv_part = N * rows_p;
     a.vn_part = rows * l.Np;
-    a.g.a = operand(w + v0 * D, rows, D, l, reinterpret_cast<uint16_t *>(ws + l.w_pack), stream);
+    uint32_t *peak = peaks ? peaks + 1 + v0 / l.piece : nullptr;
+    a.g.a = operand(w + v0 * D, rows, D, l, ws + l.w_pack, w_exp, peak, nullptr, nullptr, stream);
     int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3 grid) {
       using Tile = decltype(tile);
       grad_logits_kernel<Tile, T><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
-    transpose(w + v0 * D, static_cast<const int32_t *>(nullptr), wt, rows, D, rows_p, stream);
+    transpose<T>(w + v0 * D, nullptr, nullptr, peak, wt, rows, D, rows_p, stream);
 
     StoreArgs s{};  // dw[v, d] = sum over n of G[v, n] * h[n, d]
-    s.g.segments = l.segments;
     s.g.steps = static_cast<int32_t>(l.Np / kStepK);
     s.g.splits = l.dw_splits;
     s.g.a = GemmOperand{vn, a.vn_part, l.Np, static_cast<int32_t>(rows)};
     s.g.b = GemmOperand{ht, D * l.Np, l.Np, static_cast<int32_t>(D)};
+    s.peak = peaks;
     s.part = reinterpret_cast<float *>(ws + l.dw_part);
     s.part_stride = rows * D;
     rc = product<T>(l.dw, s, dw + v0 * D, l.dw_splits > 1, stream);
@@ -561,6 +776,8 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     s.g.a = GemmOperand{nv, a.nv_part, rows_p, static_cast<int32_t>(N)};
     s.g.b = GemmOperand{wt, D * rows_p, rows_p, static_cast<int32_t>(D)};
     s.keep = label;
+    s.factor = factor;
+    s.peak = peak;
     s.part = reinterpret_cast<float *>(ws + l.dh_part);
     s.part_stride = N * D;
     s.accumulate = v0 > 0;
@@ -648,11 +865,13 @@ int fg_linear_ce_grad(int64_t N, int64_t V, int64_t D, const void *hidden, const
   if (int rc = fg::check_space(workspace, workspace_bytes, l.bytes)) return rc;
   char *ws = static_cast<char *>(workspace);
   int32_t *label = reinterpret_cast<int32_t *>(ws + l.label);
+  uint32_t *peaks = reinterpret_cast<uint32_t *>(ws + l.peaks);
+  const int32_t n_peaks = dtype == FG_F32 ? static_cast<int32_t>(1 + l.pieces) : 0;
   const dim3 grid(static_cast<unsigned>((N + fg::kBlockThreads - 1) / fg::kBlockThreads));
   if (itype == FG_I32)
-    fg::labels_kernel<int32_t><<<grid, dim3(fg::kBlockThreads), 0, s>>>(static_cast<const int32_t *>(labels), static_cast<int32_t>(N), V, label);
+    fg::labels_kernel<int32_t><<<grid, dim3(fg::kBlockThreads), 0, s>>>(static_cast<const int32_t *>(labels), static_cast<int32_t>(N), V, label, peaks, n_peaks);
   else
-    fg::labels_kernel<int64_t><<<grid, dim3(fg::kBlockThreads), 0, s>>>(static_cast<const int64_t *>(labels), static_cast<int32_t>(N), V, label);
+    fg::labels_kernel<int64_t><<<grid, dim3(fg::kBlockThreads), 0, s>>>(static_cast<const int64_t *>(labels), static_cast<int32_t>(N), V, label, peaks, n_peaks);
 #define FG_TYPED(T)                                                                                              \
   fg::backward<T>(N, V, D, static_cast<const T *>(hidden), static_cast<const T *>(weight), lse, dloss,           \
                   static_cast<T *>(dhidden), static_cast<T *>(dweight), ws, l, s)
