@@ -38,10 +38,10 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kTop = 14;  // binary exponent that a scaled float32 operand's largest element is brought to
 
-using Big = GemmTile<256, 256, 2, 4>;   // 128 x 64 per wave, one workgroup per CU
-using Mid = GemmTile<128, 128, 2, 2>;   // 64 x 64 per wave, two workgroups per CU
-using Flat = GemmTile<64, 256, 1, 4>;   // few rows of A
-using Tall = GemmTile<256, 64, 4, 1>;   // few rows of B
+using Big = GemmTile<256, 256, 2, 4, 3>;   // 128 x 64 per wave, one workgroup per CU
+using Mid = GemmTile<128, 128, 2, 2, 3>;   // 64 x 64 per wave, two workgroups per CU
+using Flat = GemmTile<64, 256, 1, 4, 2>;   // few rows of A
+using Tall = GemmTile<256, 64, 4, 1, 2>;   // few rows of B
 
 // ------------------------------------------------------------------------------------------------ operand copies
 __device__ __forceinline__ uint32_t bits_of(float x) { return __builtin_bit_cast(uint16_t, narrow<__bf16>(x)); }
@@ -555,7 +555,7 @@ constexpr int64_t kPieceBytes = int64_t{512} << 20;  // copies and G of one piec
 struct Layout {
   int parts, segments;
   int64_t pieces;
-  bool packed;           // operands copied with k padded (float32, or rows that are no multiple of kPadK or 16 bytes)
+  bool packed;           // operands copied with k padded (float32, or rows that are no multiple of kStepK or 16 bytes)
   int64_t Dp, Np;        // D and N to multiples of 64
   int64_t piece;         // vocabulary rows per piece, a multiple of 256
   TileKind logits, dh, dw;
@@ -567,15 +567,15 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   Layout l{};
   l.parts = dtype == FG_F32 ? kParts : 1;
   l.segments = dtype == FG_F32 ? kSegments : 1;
-  l.packed = dtype == FG_F32 || D % kPadK != 0 || !aligned;
-  l.Dp = up(D, kPadK);
-  l.Np = up(N, kPadK);
+  l.packed = dtype == FG_F32 || D % kStepK != 0 || !aligned;
+  l.Dp = up(D, kStepK);
+  l.Np = up(N, kStepK);
   int64_t per_row = l.packed ? 2 * l.parts * l.Dp : 0;
   if (backward) per_row += 2 * l.parts * (2 * l.Np + D);
   const int64_t most = per_row ? std::max<int64_t>(256, kPieceBytes / per_row / 256 * 256) : up(V, 256);
   l.piece = up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), 256);  // as many pieces as needed, of equal size
   if (const int64_t rows = config().ce_piece_rows) l.piece = up(rows, 256);
-  const int64_t in_piece = std::min(l.piece, V), piece_p = up(in_piece, kPadK);
+  const int64_t in_piece = std::min(l.piece, V), piece_p = up(in_piece, kStepK);
   l.pieces = (V + l.piece - 1) / l.piece;
   l.logits = choose_tile(in_piece, N, false);
   int64_t at = 0;
@@ -743,7 +743,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   transpose(h, label, factor, peaks, ht, N, D, l.Np, stream);
   const bool dh_partial = l.dh_splits > 1 || V > l.piece;
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
-    const int64_t rows = std::min(l.piece, V - v0), rows_p = up(rows, kPadK);
+    const int64_t rows = std::min(l.piece, V - v0), rows_p = up(rows, kStepK);
     a.v0 = static_cast<int32_t>(v0);
     a.pitch_v = static_cast<int32_t>(rows_p);
     a.nv_part = N * rows_p;

@@ -8,14 +8,17 @@
 // first, then, after the sum is multiplied by 2^-11, hi * hi; lo * lo is at most 2^-24 of the terms.  That is float32's
 // accuracy at a third of the 16-bit rate, 5.3 times the peak rate of the float32 matrix instructions.
 //
-// A workgroup computes a BM x BN tile in steps of 32 k.  The operands' rows go straight to LDS (16 bytes per lane, no
-// registers in between) into one of four stages, three steps ahead; the fragments of a step's first half are read
-// while the step before it still multiplies, so that a wave never waits for LDS with nothing to issue.  A tile row is
-// 64 bytes in LDS; its four 16-byte pieces are placed at (piece ^ (row / 4 % 4)), so that the lanes of a fragment read,
-// which take the same piece of consecutive rows, spread over all banks.  The permutation is applied on the way in, by
-// what each lane fetches.  Rows past the operands' ends are read as the last row and dropped by the epilogues; k is a
+// A workgroup computes a BM x BN tile in steps of 64 k.  The operands' rows go straight to LDS (16 bytes per lane, whole
+// 128-byte lines, no registers in between) into one of two stages.  The fragments of each quarter of a step are read
+// while the quarter before it multiplies, over the border of the steps too: the waves meet before the last quarter, when
+// its fragments are in registers, the next stage has arrived and this one can be filled again.  A tile row is 128 bytes
+// in LDS; its eight 16-byte pieces are placed at (piece ^ (row / 2 % 8)), so that the lanes of a fragment read, which
+// take the same piece of consecutive rows, spread over all banks.  The permutation is applied on the way in, by what
+// each lane fetches.  Rows past the operands' ends are read as the last row and dropped by the epilogues; k is a
 // multiple of 64 (padded copies hold zeros there).
 #pragma once
+
+#include <type_traits>
 
 #include "element.hpp"
 
@@ -25,9 +28,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr int kPadK = 64;     // k is padded to a multiple of this
-constexpr int kStepK = 32;    // k of one stage
-constexpr int kStages = 4;
+constexpr int kStepK = 64;    // k of one stage; k is padded to a multiple of this
 constexpr int kParts = 2;     // float16 parts of a float32
 constexpr int kSegments = 3;  // products of parts that are added
 constexpr int kLowBits = 11;  // lo is kept times 2^kLowBits
@@ -72,19 +73,23 @@ struct GemmShape {
   int32_t tiles_m = 0, tiles_n = 0;
 };
 
-template <int BM_, int BN_, int WM_, int WN_>
+template <int BM_, int BN_, int WM_, int WN_, int kStagesA_>
 struct GemmTile {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, kStagesA = kStagesA_;
   static constexpr int kWaves = WM * WN, kThreads = kWaves * kWaveSize;
   static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;                  // 32 x 32 blocks of one wave
-  static constexpr int kLoadsA = BM / 16 / kWaves, kLoadsB = BN / 16 / kWaves;  // 16 rows of 64 bytes per wave and load
-  static constexpr int kStage = (BM + BN) * kStepK;                           // elements of one stage
-  static constexpr int kLds = kStages * kStage;
-  static_assert(kLoadsA * 16 * kWaves == BM && kLoadsB * 16 * kWaves == BN, "rows divide over the waves");
+  static constexpr int kLoadsA = BM / 8 / kWaves, kLoadsB = BN / 8 / kWaves;  // 8 rows of 128 bytes per wave and load
+  static constexpr int kStageA = BM * kStepK, kStageB = BN * kStepK;          // elements of one stage
+  static constexpr int kLds = kStagesA * kStageA + 2 * kStageB;
+  static_assert(kStagesA == 2 || kStagesA == 3);
+  static_assert(kLds * 2 <= 163840, "the LDS of a CU");
+  static_assert(kLoadsA * 8 * kWaves == BM && kLoadsB * 8 * kWaves == BN, "rows divide over the waves");
 };
 
 // Where this workgroup works: tile and share of k.  Workgroup id x runs on die x % 8; the ids of one die are mapped
-// to consecutive tiles, n fastest, so that each die's L2 keeps the operand rows its tiles share.
+// to consecutive tiles, and those run down kGroupM tiles of m before n moves on: the 32 workgroups that a die runs at a
+// time then share 8 tiles' rows of A and 4 of B, which its L2 fetches once.
+constexpr uint32_t kGroupM = 8;
 struct GemmPlace {
   int32_t tm, tn, split;
 };
@@ -96,8 +101,10 @@ __device__ __forceinline__ GemmPlace gemm_place(const GemmShape &g) {
   GemmPlace p;
   p.split = static_cast<int32_t>(id / tiles);
   const uint32_t t = id - p.split * tiles;
-  p.tm = static_cast<int32_t>(t / g.tiles_n);
-  p.tn = static_cast<int32_t>(t - static_cast<uint32_t>(p.tm) * g.tiles_n);
+  const uint32_t band = t / (kGroupM * g.tiles_n), in_band = t - band * kGroupM * g.tiles_n;
+  const uint32_t height = min(kGroupM, static_cast<uint32_t>(g.tiles_m) - band * kGroupM);
+  p.tn = static_cast<int32_t>(in_band / height);
+  p.tm = static_cast<int32_t>(band * kGroupM + in_band - p.tn * height);
   return p;
 }
 
@@ -134,66 +141,100 @@ __device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &a
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc.c[i][j][r] = 0.0f;
 
-  // what this lane fetches: row lane / 4 of the sixteen of a load, the piece that belongs at place lane % 4
+  // what this lane fetches: row lane / 8 of the eight of a load, the piece that belongs at place lane % 8
   const int64_t m0 = static_cast<int64_t>(at.tm) * Tile::BM, n0 = static_cast<int64_t>(at.tn) * Tile::BN;
   const int rows_a = static_cast<int>(min<int64_t>(Tile::BM, g.a.rows - m0));
   const int rows_b = static_cast<int>(min<int64_t>(Tile::BN, g.b.rows - n0));
   const uint32_t pitch_a = static_cast<uint32_t>(g.a.pitch) * 2, pitch_b = static_cast<uint32_t>(g.b.pitch) * 2;
-  const uint32_t piece_in = ((lane % 4) ^ ((lane >> 4) & 3)) * 16;  // row / 4 % 4 = lane / 16
   uint32_t off_a[Tile::kLoadsA], off_b[Tile::kLoadsB];
 #pragma unroll
-  for (int j = 0; j < Tile::kLoadsA; ++j)
-    off_a[j] = min((wave + j * Tile::kWaves) * 16 + lane / 4, rows_a - 1) * pitch_a + piece_in;
+  for (int j = 0; j < Tile::kLoadsA; ++j) {
+    const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
+    off_a[j] = min(row, rows_a - 1) * pitch_a + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
+  }
 #pragma unroll
-  for (int j = 0; j < Tile::kLoadsB; ++j)
-    off_b[j] = min((wave + j * Tile::kWaves) * 16 + lane / 4, rows_b - 1) * pitch_b + piece_in;
+  for (int j = 0; j < Tile::kLoadsB; ++j) {
+    const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
+    off_b[j] = min(row, rows_b - 1) * pitch_b + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
+  }
   const uint32_t bytes_a = rows_a * pitch_a, bytes_b = rows_b * pitch_b;
 
   const int total = g.steps * M::kSegments;
   const int first = static_cast<int>(static_cast<int64_t>(total) * at.split / g.splits);
   const int last = static_cast<int>(static_cast<int64_t>(total) * (at.split + 1) / g.splits);
-  // the next load's parts and step: segment 0 is hi * lo, 1 is lo * hi, 2 (or the only one) hi * hi
-  int seg = first / g.steps, step = first - seg * g.steps;
-  auto load = [&](int i) {
-    const uint16_t *pa = g.a.p + (M::kSegments == 3 && seg == 1 ? g.a.part : 0) + m0 * g.a.pitch;
-    const uint16_t *pb = g.b.p + (M::kSegments == 3 && seg == 0 ? g.b.part : 0) + n0 * g.b.pitch;
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(pa), 0, bytes_a, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(pb), 0, bytes_b, 0x00020000);
-    const int k = step * (kStepK * 2);
-    uint16_t *base = lds + (i & (kStages - 1)) * Tile::kStage;
-#pragma unroll
-    for (int j = 0; j < Tile::kLoadsA; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (LdsPtr)(base + (wave + j * Tile::kWaves) * 16 * kStepK), 16, off_a[j], k, 0, 0);
-#pragma unroll
-    for (int j = 0; j < Tile::kLoadsB; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rb, (LdsPtr)(base + (Tile::BM + (wave + j * Tile::kWaves) * 16) * kStepK), 16, off_b[j], k, 0, 0);
-    if (++step == g.steps) {
-      step = 0;
-      ++seg;
+  // Loads of one step of an operand: its parts (segment 0 is hi * lo, 1 is lo * hi, 2 or the only one hi * hi), its k and
+  // its stage.  Past the last step nothing is fetched (no bytes are in range), so that the loop has no branches around
+  // its loads and always the same number of them under way.
+  struct Cursor {
+    int seg, step, slot, left;
+  };
+  const int n = last - first;
+  Cursor ca{first / g.steps, first % g.steps, 0, n}, cb = ca;
+  auto advance = [&](Cursor &c, int stages) {
+    --c.left;
+    if (++c.step == g.steps) {
+      c.step = 0;
+      ++c.seg;
     }
+    if (++c.slot == stages) c.slot = 0;
+  };
+  uint16_t *const lds_b = lds + Tile::kStagesA * Tile::kStageA;
+  auto load_a = [&](int j) {
+    const uint16_t *p = g.a.p + (M::kSegments == 3 && ca.seg == 1 ? g.a.part : 0) + m0 * g.a.pitch;
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, ca.left > 0 ? bytes_a : 0, 0x00020000);
+    uint16_t *to = lds + ca.slot * Tile::kStageA + (wave + j * Tile::kWaves) * 8 * kStepK;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_a[j], ca.step * (kStepK * 2), 0, 0);
+  };
+  auto load_b = [&](int j) {
+    const uint16_t *p = g.b.p + (M::kSegments == 3 && cb.seg == 0 ? g.b.part : 0) + n0 * g.b.pitch;
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, cb.left > 0 ? bytes_b : 0, 0x00020000);
+    uint16_t *to = lds_b + cb.slot * Tile::kStageB + (wave + j * Tile::kWaves) * 8 * kStepK;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_b[j], cb.step * (kStepK * 2), 0, 0);
+  };
+  // One period of loads, from one meeting of the waves to the next: B's next step, then A's next (the one after, where A
+  // has three stages).  They are issued a few at a time between the matrix instructions of the period's first kQuarters
+  // quarters: all at once they would fill the queue and hold the waves up.
+  constexpr bool kDeep = Tile::kStagesA == 3;
+  constexpr int kQuarters = kDeep ? 4 : 2, kPerQuarter = (kLoads + kQuarters - 1) / kQuarters;
+  auto load_one = [&](int l) {
+    if (l < Tile::kLoadsB) load_b(l);
+    else if (l < kLoads) load_a(l - Tile::kLoadsB);
+    if (l == Tile::kLoadsB - 1) advance(cb, 2);
+    if (l == kLoads - 1) advance(ca, Tile::kStagesA);
   };
 
-  // fragments: lane l holds row l % 32, eight k from 16 * half + 8 * (l / 32) on
+  // fragments: lane l holds row l % 32, eight k from 16 * quarter + 8 * (l / 32) on
   const int row_a = wm * (Tile::BM / Tile::WM) + lane % 32, row_b = wn * (Tile::BN / Tile::WN) + lane % 32;
-  const int twist = (lane >> 2) & 3;
-  const int at_a = row_a * kStepK, at_b = (Tile::BM + row_b) * kStepK;
-  const int half0 = ((lane / 32) ^ twist) * 8, half1 = ((2 + lane / 32) ^ twist) * 8;
+  const int at_a = row_a * kStepK, at_b = row_b * kStepK;
+  const int twist = (lane >> 1) & 7;
   struct Fragments {
     bf16x8 a[Tile::TM], b[Tile::TN];
   };
-  auto read = [&](Fragments &f, int i, int half) {
-    const uint16_t *s = lds + (i & (kStages - 1)) * Tile::kStage + half;
+  int slot_a = 0, slot_b = 0;  // of the step that is read
+  auto read = [&](Fragments &f, int quarter) {
+    const int piece = ((2 * quarter + lane / 32) ^ twist) * 8;
+    const uint16_t *sa = lds + slot_a * Tile::kStageA + at_a + piece, *sb = lds_b + slot_b * Tile::kStageB + at_b + piece;
 #pragma unroll
-    for (int t = 0; t < Tile::TM; ++t) f.a[t] = *reinterpret_cast<const bf16x8 *>(s + at_a + t * 32 * kStepK);
+    for (int t = 0; t < Tile::TM; ++t) f.a[t] = *reinterpret_cast<const bf16x8 *>(sa + t * 32 * kStepK);
 #pragma unroll
-    for (int t = 0; t < Tile::TN; ++t) f.b[t] = *reinterpret_cast<const bf16x8 *>(s + at_b + t * 32 * kStepK);
+    for (int t = 0; t < Tile::TN; ++t) f.b[t] = *reinterpret_cast<const bf16x8 *>(sb + t * 32 * kStepK);
   };
-  auto multiply = [&](const Fragments &f) {
+  // kQuarter of the period, whose share of the loads goes out between the products
+  auto multiply = [&](const Fragments &f, auto quarter) {
+    constexpr int kQuarter = decltype(quarter)::value, kProducts = Tile::TM * Tile::TN;
+    constexpr int kShare = kQuarter < kQuarters ? kPerQuarter : 0;
+    __builtin_amdgcn_sched_barrier(0);  // the reads before it are under way
 #pragma unroll
-    for (int t = 0; t < Tile::TM; ++t)
+    for (int p = 0; p < kProducts; ++p) {
+      const int t = p / Tile::TN, u = p % Tile::TN;
+      acc.c[t][u] = M::mfma(f.a[t], f.b[u], acc.c[t][u]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int u = 0; u < Tile::TN; ++u) acc.c[t][u] = M::mfma(f.a[t], f.b[u], acc.c[t][u]);
+      for (int l = kShare * p / kProducts; l < kShare * (p + 1) / kProducts; ++l) load_one(kQuarter * kPerQuarter + l);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
   auto lower = [&]() {
 #pragma unroll
@@ -204,30 +245,44 @@ __device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &a
         for (int r = 0; r < 16; ++r) acc.c[t][u][r] *= 1.0f / (1 << kLowBits);
   };
 
-  const int n = last - first;
+  using Q0 = std::integral_constant<int, 0>;
+  using Q1 = std::integral_constant<int, 1>;
+  using Q2 = std::integral_constant<int, 2>;
+  using Q3 = std::integral_constant<int, 3>;
   const int cross = M::kSegments == 3 ? 2 * g.steps - first : 0;  // steps of this share before hi * hi begins
-  if (n > 0) {
-    load(0);
-    if (n > 1) load(1);
-    if (n > 2) load(2);
-    Fragments f0, f1;
-    // step 0 has arrived (its loads are the oldest)
-    if (n > 2) arrive_and_meet<2 * kLoads>();
-    else arrive_and_meet<0>();
-    read(f0, 0, half0);
-    for (int i = 0; i < n; ++i) {
-      // step i + 1 has arrived for every wave, and nobody reads step i - 1 any more, whose stage step i + 3 takes
-      if (i + 2 < n) arrive_and_meet<kLoads>();
-      else arrive_and_meet<0>();
-      if (i + 3 < n) load(i + 3);
-      if (M::kSegments == 3 && i > 0 && i == cross) lower();
-      read(f1, i, half1);
-      multiply(f0);
-      if (i + 1 < n) read(f0, i + 1, half0);
-      multiply(f1);
-    }
-    if (M::kSegments == 3 && cross >= n) lower();
+  Fragments f0, f1;
+#pragma unroll
+  for (int j = 0; j < Tile::kLoadsA; ++j) load_a(j);
+  advance(ca, Tile::kStagesA);
+#pragma unroll
+  for (int j = 0; j < Tile::kLoadsB; ++j) load_b(j);
+  advance(cb, 2);
+  if constexpr (kDeep) {
+#pragma unroll
+    for (int j = 0; j < Tile::kLoadsA; ++j) load_a(j);
+    advance(ca, Tile::kStagesA);
   }
+#pragma unroll
+  for (int l = 0; l < kPerQuarter; ++l) load_one(l);
+  arrive_and_meet<kPerQuarter + (kDeep ? Tile::kLoadsA : 0)>();
+  read(f0, 0);
+  for (int i = 0; i < n; ++i) {
+    if (M::kSegments == 3 && i > 0 && i == cross) lower();
+    read(f1, 1);
+    multiply(f0, Q1{});
+    read(f0, 2);
+    multiply(f1, Q2{});
+    read(f1, 3);
+    multiply(f0, Q3{});
+    // the next step is there for every wave (only A's step after it may still be on its way), nobody reads this one
+    arrive_and_meet<kDeep ? Tile::kLoadsA : 0>();
+    if (++slot_a == Tile::kStagesA) slot_a = 0;
+    slot_b ^= 1;
+    read(f0, 0);  // past the last step: what is read is not used
+    multiply(f1, Q0{});
+  }
+  if (M::kSegments == 3 && cross >= n) lower();
+  arrive_and_meet<0>();  // the epilogue may use the LDS
 #endif
 }
 
