@@ -171,17 +171,19 @@ __global__ __launch_bounds__(kBlockThreads) void labels_kernel(const Id *labels,
 }
 
 // ------------------------------------------------------------------------------------------------ forward
+// Statistics of a set of logits: {r, s} with s = sum of exp(l) / 2^r, r a whole number at or just above the largest
+// logit / ln 2.  A whole r is exact, so exp2(l * log2(e) - r) is one multiply-add, rounded once, near the terms that count.
 struct StatsArgs {
   GemmShape g;             // a: rows of w, b: h
   const int32_t *exp_a, *exp_b;  // float32: exponents of the rows
-  float2 *part;            // [tiles of vocabulary, N]: largest logit, sum of exp(l - largest)
+  float2 *part;            // [tiles of vocabulary, N]
   int32_t tile0;           // first tile of this piece
 };
 
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
-  const float m = fmaxf(a.x, b.x);
-  if (m == -INFINITY) return float2{m, a.y + b.y};
-  return float2{m, a.y * __builtin_amdgcn_exp2f((a.x - m) * kLog2e) + b.y * __builtin_amdgcn_exp2f((b.x - m) * kLog2e)};
+  const float r = fmaxf(a.x, b.x);
+  if (r == -INFINITY) return float2{r, a.y + b.y};
+  return float2{r, a.y * __builtin_amdgcn_exp2f(a.x - r) + b.y * __builtin_amdgcn_exp2f(b.x - r)};
 }
 
 // Takes the rows' exponents back out of the accumulators: what is left are the logits.
@@ -244,13 +246,13 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
     for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) m = fmaxf(m, acc.c[i][j][r]);
-    m = fmaxf(m, __shfl_xor(m, 32, kWaveSize));
+    m = __builtin_ceilf(fmaxf(m, __shfl_xor(m, 32, kWaveSize)) * kLog2e);
     const float from = m == -INFINITY ? 0.0f : m;
     float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f((acc.c[i][j][r] - from) * kLog2e);
+      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][r], kLog2e, -from));
     s += __shfl_xor(s, 32, kWaveSize);
     if (lane < 32) stats[wm * Tile::BN + wn * (Tile::BN / Tile::WN) + 32 * j + lane] = float2{m, s};
   }
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(kThreads) void loss_kernel(const float2 *part, int3
     if (share < half) joined[share][row] = s = join_stats(s, joined[share + half][row]);
   }
   if (share == 0) {
-    const float r = s.x + logf(s.y);
+    const float r = static_cast<float>((static_cast<double>(s.x) + log2(static_cast<double>(s.y))) * 0.69314718055994530942);
     row_lse[row] = r;
     if (n0 + row < N) lse[n0 + row] = r;
   }
@@ -354,24 +356,38 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
   const int v0 = at.tm * Tile::BM + wave_v;
   const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wave_n;
   to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
-  const bool edge = v0 + Tile::BM / Tile::WM > a.g.a.rows;
+  // P = exp2(l * log2(e) - r) * 2^(r - lse * log2(e)) with a whole r: the first factor is one multiply-add, rounded once,
+  // the second one is taken per row, in double, together with what P is stored times.
 #pragma unroll
   for (int j = 0; j < Tile::TN; ++j) {
     const int64_t n = n0 + 32 * j + lane % 32;
     const int32_t label = n < a.g.b.rows ? a.label[n] : -1;
-    const float lse = label >= 0 ? a.lse[n] : 0.0f;
-    const float times = sizeof(T) == 4 ? static_cast<float>(1 << kTop) : label >= 0 ? a.dloss[n] : 0.0f;
+    const float times = label < 0 ? 0.0f : sizeof(T) == 4 ? static_cast<float>(1 << kTop) : a.dloss[n];
+    const double lse2 = label < 0 ? 0.0 : static_cast<double>(a.lse[n]) * 1.44269504088896340736;
+    const float r = static_cast<float>(rint(lse2));
+    const float scale = times * __builtin_amdgcn_exp2f(static_cast<float>(static_cast<double>(r) - lse2));
     const int32_t hit = label >= 0 ? label - a.v0 - v0 : -1;  // row of this wave's block that is the label's
-    const bool any_hit = __any(hit >= 0 && hit < Tile::BM / Tile::WM);
 #pragma unroll
     for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int v = 32 * i + acc_row(r, lane);
-        float p = __builtin_amdgcn_exp2f((acc.c[i][j][r] - lse) * kLog2e);
-        if (any_hit && v == hit) p -= 1.0f;
-        acc.c[i][j][r] = label >= 0 && !(edge && v0 + v >= a.g.a.rows) ? p * times : 0.0f;
+      for (int k = 0; k < 16; ++k) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][k], kLog2e, -r)) * scale;
+        acc.c[i][j][k] = label >= 0 ? p : 0.0f;
       }
+    if (__any(hit >= 0 && hit < Tile::BM / Tile::WM)) {
+#pragma unroll
+      for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (32 * i + acc_row(k, lane) == hit) acc.c[i][j][k] -= times;
+    }
+    if (v0 + Tile::BM / Tile::WM > a.g.a.rows) {  // rows past the end are the last row again
+#pragma unroll
+      for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+        for (int k = 0; k < 16; ++k)
+          if (v0 + 32 * i + acc_row(k, lane) >= a.g.a.rows) acc.c[i][j][k] = 0.0f;
+    }
   }
   constexpr int kPieces = Tile::BM / 8;  // of 16 bytes in a row of the [n, v] tile
   auto place = [](int n, int piece) { return piece ^ (kPieces == 8 ? (n >> 1) & 7 : n & (kPieces - 1)); };
@@ -384,43 +400,51 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
     }
     return bits;
   };
+  const int64_t first_n = static_cast<int64_t>(at.tn) * Tile::BN;
+  const int first_v = at.tm * Tile::BM;
+  const bool whole = first_v + Tile::BM <= a.g.a.rows && first_n + Tile::BN <= a.g.b.rows;
+  auto store = [&](auto inside, int part) {  // inside: the whole tile lies within the matrix
+    constexpr bool kInside = decltype(inside)::value;
 #pragma unroll
-  for (int part = 0; part < Multiply<T>::kParts; ++part) {
-    __syncthreads();  // the operands, or the first part, are no longer read
-#pragma unroll
-    for (int j = 0; j < Tile::TN; ++j)
+    for (int j = 0; j < Tile::TN; ++j) {
+      const int64_t col = n0 + 32 * j + lane % 32 / 4 * 4;
+      const int n = wave_n + 32 * j + lane % 32;
 #pragma unroll
       for (int i = 0; i < Tile::TM; ++i) {
         FG_IN_ORDER();
+        uint16_t *to = a.vn + part * a.vn_part + static_cast<int64_t>(v0 + 32 * i + acc_row(0, lane) + lane % 4) * a.pitch_n + col;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          uint2 x;
           float e[4] = {acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
+          uint2 x;
           x.x = take(e[0]);
           x.x |= take(e[1]) << 16;
           x.y = take(e[2]);
           x.y |= take(e[3]) << 16;
 #pragma unroll
           for (int k = 0; k < 4; ++k) acc.c[i][j][4 * q + k] = e[k];
-          const int n = wave_n + 32 * j + lane % 32, v = wave_v + 32 * i + 8 * q;  // lanes 32..63: the second half
+          const int v = wave_v + 32 * i + 8 * q;  // lanes 32..63: the second half of the piece
           *reinterpret_cast<uint2 *>(lds + n * Tile::BM + place(n, v / 8) * 8 + lane / 32 * 4) = x;
           const uint2 y = turn4(x, lane);
-          const int row = v0 + 32 * i + acc_row(4 * q, lane) + lane % 4;
-          const int64_t col = n0 + 32 * j + lane % 32 / 4 * 4;
-          if (row < a.g.a.rows && col < a.pitch_n)
-            *reinterpret_cast<uint2 *>(a.vn + part * a.vn_part + static_cast<int64_t>(row) * a.pitch_n + col) = y;
+          if (kInside || (v0 + 32 * i + acc_row(4 * q, lane) + lane % 4 < a.g.a.rows && col < a.pitch_n))
+            *reinterpret_cast<uint2 *>(to + static_cast<int64_t>(8 * q) * a.pitch_n) = y;
         }
       }
+    }
     __syncthreads();
-    const int64_t first_n = static_cast<int64_t>(at.tn) * Tile::BN;
-    const int first_v = at.tm * Tile::BM;
 #pragma unroll 4
     for (int t = threadIdx.x; t < Tile::BN * kPieces; t += Tile::kThreads) {
       const int n = t / kPieces, piece = t % kPieces;
-      if (first_n + n < a.g.b.rows && first_v + piece * 8 < a.pitch_v)
+      if (kInside || (first_n + n < a.g.b.rows && first_v + piece * 8 < a.pitch_v))
         *reinterpret_cast<uint4 *>(a.nv + part * a.nv_part + (first_n + n) * a.pitch_v + first_v + piece * 8) =
             *reinterpret_cast<const uint4 *>(lds + n * Tile::BM + place(n, piece) * 8);
     }
+  };
+#pragma unroll
+  for (int part = 0; part < Multiply<T>::kParts; ++part) {
+    if (part) __syncthreads();  // the first part is no longer read
+    if (sizeof(T) == 2 && whole) store(std::true_type{}, part);  // a second copy of the code costs float32 its registers
+    else store(std::false_type{}, part);
   }
 }
 
