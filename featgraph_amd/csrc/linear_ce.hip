@@ -546,6 +546,10 @@ constexpr TileSize kTileSize[] = {{256, 256, 1, 1.0}, {128, 128, 2, 0.7}, {64, 2
 constexpr int kCus = 256;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t steps_of(int64_t k) { return (k + kStepK - 1) / kStepK; }
+// Elements from one row of a copy to the next: an odd number of 128-byte lines, so that the lines which a tile's rows need
+// at the same k do not all belong to the same few channels of the caches.
+int64_t pitch_of(int64_t k) { return (steps_of(k) | 1) * kStepK; }
 
 // The tile whose rounds of workgroups over the device take the least time; tiles that can share a long k among
 // several workgroups (`splittable`) are judged by their total work instead.
@@ -580,7 +584,7 @@ struct Layout {
   int parts, segments;
   int64_t pieces;
   bool packed;           // operands copied with k padded (float32, or rows that are no multiple of kStepK or 16 bytes)
-  int64_t Dp, Np;        // D and N to multiples of 64
+  int64_t Dp, Np;        // pitches of rows of D and N elements
   int64_t piece;         // vocabulary rows per piece, a multiple of 256
   TileKind logits, dh, dw;
   int dh_splits, dw_splits;
@@ -592,14 +596,14 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   l.parts = dtype == FG_F32 ? kParts : 1;
   l.segments = dtype == FG_F32 ? kSegments : 1;
   l.packed = dtype == FG_F32 || D % kStepK != 0 || !aligned;
-  l.Dp = up(D, kStepK);
-  l.Np = up(N, kStepK);
+  l.Dp = pitch_of(D);
+  l.Np = pitch_of(N);
   int64_t per_row = l.packed ? 2 * l.parts * l.Dp : 0;
   if (backward) per_row += 2 * l.parts * (2 * l.Np + D);
   const int64_t most = per_row ? std::max<int64_t>(256, kPieceBytes / per_row / 256 * 256) : up(V, 256);
   l.piece = up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), 256);  // as many pieces as needed, of equal size
   if (const int64_t rows = config().ce_piece_rows) l.piece = up(rows, 256);
-  const int64_t in_piece = std::min(l.piece, V), piece_p = up(in_piece, kStepK);
+  const int64_t in_piece = std::min(l.piece, V), piece_p = pitch_of(in_piece);
   l.pieces = (V + l.piece - 1) / l.piece;
   l.logits = choose_tile(in_piece, N, false);
   int64_t at = 0;
@@ -621,8 +625,8 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   } else {
     l.dh = choose_tile(N, D, true);
     l.dw = choose_tile(in_piece, D, true);
-    l.dh_splits = choose_splits(l.dh, N, D, piece_p / kStepK * l.segments);
-    l.dw_splits = choose_splits(l.dw, in_piece, D, l.Np / kStepK * l.segments);
+    l.dh_splits = choose_splits(l.dh, N, D, steps_of(in_piece) * l.segments);
+    l.dw_splits = choose_splits(l.dw, in_piece, D, steps_of(N) * l.segments);
     l.label = take(4 * N);
     l.ht = take(2 * l.parts * D * l.Np);
     l.wt = take(2 * l.parts * D * piece_p);
@@ -700,7 +704,7 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
             char *ws, const Layout &l, hipStream_t stream) {
   StatsArgs a{};
   a.part = reinterpret_cast<float2 *>(ws + l.stats);
-  a.g.steps = static_cast<int32_t>(l.Dp / kStepK);
+  a.g.steps = static_cast<int32_t>(steps_of(D));
   auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
   a.exp_a = w_exp;
   a.exp_b = h_exp;
@@ -757,7 +761,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   a.nv = nv;
   a.vn = vn;
   a.pitch_n = static_cast<int32_t>(l.Np);
-  a.g.steps = static_cast<int32_t>(l.Dp / kStepK);
+  a.g.steps = static_cast<int32_t>(steps_of(D));
   auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
   uint32_t *peaks = sizeof(T) == 4 ? reinterpret_cast<uint32_t *>(ws + l.peaks) : nullptr;  // of h, then of each piece of w
   const float *factor = sizeof(T) == 4 ? dloss : nullptr;
@@ -767,7 +771,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   transpose(h, label, factor, peaks, ht, N, D, l.Np, stream);
   const bool dh_partial = l.dh_splits > 1 || V > l.piece;
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
-    const int64_t rows = std::min(l.piece, V - v0), rows_p = up(rows, kStepK);
+    const int64_t rows = std::min(l.piece, V - v0), rows_p = pitch_of(rows);
     a.v0 = static_cast<int32_t>(v0);
     a.pitch_v = static_cast<int32_t>(rows_p);
     a.nv_part = N * rows_p;
@@ -782,7 +786,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     transpose<T>(w + v0 * D, nullptr, nullptr, peak, wt, rows, D, rows_p, stream);
 
     StoreArgs s{};  // dw[v, d] = sum over n of G[v, n] * h[n, d]
-    s.g.steps = static_cast<int32_t>(l.Np / kStepK);
+    s.g.steps = static_cast<int32_t>(steps_of(N));
     s.g.splits = l.dw_splits;
     s.g.a = GemmOperand{vn, a.vn_part, l.Np, static_cast<int32_t>(rows)};
     s.g.b = GemmOperand{ht, D * l.Np, l.Np, static_cast<int32_t>(D)};
@@ -795,7 +799,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
       join_kernel<T><<<dim3(flat_grid(rows * D)), dim3(kBlockThreads), 0, stream>>>(
           s.part, s.part_stride, l.dw_splits, dw + v0 * D, rows, static_cast<int32_t>(D), nullptr);
 
-    s.g.steps = static_cast<int32_t>(rows_p / kStepK);  // dh[n, d] = sum over v of G[n, v] * w[v, d]
+    s.g.steps = static_cast<int32_t>(steps_of(rows));  // dh[n, d] = sum over v of G[n, v] * w[v, d]
     s.g.splits = l.dh_splits;
     s.g.a = GemmOperand{nv, a.nv_part, rows_p, static_cast<int32_t>(N)};
     s.g.b = GemmOperand{wt, D * rows_p, rows_p, static_cast<int32_t>(D)};
