@@ -67,6 +67,16 @@ __device__ __forceinline__ int exponent_for(uint32_t peak) {
   return min(126, max(-126, kTop - (static_cast<int>(peak >> 23) - 127)));
 }
 
+// The largest element of a matrix is collected in kPeakSlots words of lines of their own, by workgroup: one word would
+// serialise the workgroups.
+constexpr int kPeakSlots = 64, kPeakStride = 32;
+__device__ __forceinline__ uint32_t read_peak(const uint32_t *peak) {
+  uint32_t m = peak[(threadIdx.x & (kPeakSlots - 1)) * kPeakStride];
+#pragma unroll
+  for (int d = 1; d < kWaveSize; d <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), d, kWaveSize)));
+  return m;
+}
+
 __device__ __forceinline__ uint32_t finite_bits(float x) {
   const uint32_t u = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
   return u < 0x7f800000u ? u : 0u;
@@ -113,7 +123,7 @@ __global__ __launch_bounds__(kBlockThreads) void split_rows_kernel(const float *
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kWavesPerBlock; ++w) most = max(most, peaks[w]);
-    atomicMax(peak, most);  // a largest value does not depend on the order
+    atomicMax(peak + blockIdx.x % kPeakSlots * kPeakStride, most);  // a largest value does not depend on the order
   }
 }
 
@@ -128,7 +138,7 @@ __global__ __launch_bounds__(kBlockThreads) void transpose_kernel(const T *x, co
   __shared__ float tile[64][65];
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
   const int c0 = blockIdx.y * 64;
-  const int e = peak ? exponent_for(*peak) : 0;
+  const int e = peak ? exponent_for(read_peak(peak)) : 0;
   const int c = c0 + threadIdx.x % kLanes * kVec;
   for (int k = threadIdx.x / kLanes; k < 64; k += kBlockThreads / kLanes) {
     const int64_t r = r0 + k;
@@ -176,8 +186,12 @@ __global__ __launch_bounds__(kBlockThreads) void labels_kernel(const Id *labels,
 struct StatsArgs {
   GemmShape g;             // a: rows of w, b: h
   const int32_t *exp_a, *exp_b;  // float32: exponents of the rows
-  float2 *part;            // [tiles of vocabulary, N]
-  int32_t tile0;           // first tile of this piece
+  float2 *part;            // [ranges of vocabulary, N]
+  int32_t ranges;          // that the tiles of vocabulary of this piece are divided into
+  int32_t range0;          // first of them
+  const void *labels;      // [N]
+  int64_t v0;              // first vocabulary row of this piece
+  float *label_logit;      // [N], written where the label's row is met
 };
 
 __device__ __forceinline__ float2 join_stats(float2 a, float2 b) {
@@ -218,43 +232,80 @@ __device__ __forceinline__ void to_logits(GemmAcc<Tile> &acc, const int32_t *exp
   }
 }
 
-template <typename Tile, typename T>
+// A workgroup takes one tile of rows n and a range of the vocabulary, tile after tile without a pause in its loads; each
+// lane keeps the statistics of the logits it meets (its column n, half the rows of its wave) until the end.
+template <typename Tile, typename T, typename Id>
 __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
-  const GemmPlace at = gemm_place(a.g);
-  gemm_tile<Tile, T>(a.g, at, lds, acc);
-  __syncthreads();
+  const uint32_t die = blockIdx.x % kXcds, q = gridDim.x / kXcds;  // consecutive ids on one die, as in gemm_place
+  const uint32_t id = die * q + min<uint32_t>(die, gridDim.x % kXcds) + blockIdx.x / kXcds;
+  const int range = static_cast<int>(id / a.g.tiles_n);
+  GemmPlace at;
+  at.split = 0;
+  at.tn = static_cast<int32_t>(id - static_cast<uint32_t>(range) * a.g.tiles_n);
+  at.tm = static_cast<int32_t>(static_cast<int64_t>(a.g.tiles_m) * range / a.ranges);
+  const int tiles = static_cast<int>(static_cast<int64_t>(a.g.tiles_m) * (range + 1) / a.ranges) - at.tm;
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
-  const int v0 = at.tm * Tile::BM + wm * (Tile::BM / Tile::WM);
   const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wn * (Tile::BN / Tile::WN);
-  to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
-  float2 *stats = reinterpret_cast<float2 *>(lds);  // [WM][BN]
-  const bool edge = v0 + Tile::BM / Tile::WM > a.g.a.rows;
+  const int64_t first_v = static_cast<int64_t>(at.tm) * Tile::BM + wm * (Tile::BM / Tile::WM);
+  float top[Tile::TN], sum[Tile::TN];
+  int64_t label[Tile::TN];  // row of the piece that is the label's, relative to this wave's first
 #pragma unroll
   for (int j = 0; j < Tile::TN; ++j) {
-    if (edge) {
+    const int64_t n = n0 + 32 * j + lane % 32;
+    top[j] = -INFINITY;
+    sum[j] = 0.0f;
+    label[j] = n < a.g.b.rows ? static_cast<int64_t>(static_cast<const Id *>(a.labels)[n]) - a.v0 - first_v : -1;
+  }
+  gemm_tiles<Tile, T>(a.g, at, tiles, lds, acc, [&](int tile) {
+    const int64_t v0 = first_v + static_cast<int64_t>(tile) * Tile::BM;
+    to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
+#pragma unroll
+    for (int j = 0; j < Tile::TN; ++j) {
+      if (v0 + Tile::BM / Tile::WM > a.g.a.rows) {
+        const int end = static_cast<int>(max<int64_t>(a.g.a.rows - v0, 0)) - acc_row(0, lane);
+#pragma unroll
+        for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * i + acc_row(r, 0) >= end) acc.c[i][j][r] = -INFINITY;
+      }
+      const int64_t past = label[j] - static_cast<int64_t>(tile) * Tile::BM;
+      const int hit = past >= 0 && past < Tile::BM / Tile::WM && v0 + past < a.g.a.rows ? static_cast<int>(past) : -1;
+      if (__any(hit >= 0)) {
+        float logit = 0.0f;
+        const int mine = hit - acc_row(0, lane);
+#pragma unroll
+        for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) logit = 32 * i + acc_row(r, 0) == mine ? acc.c[i][j][r] : logit;
+        if (hit >= 0 && hit / 4 % 2 == lane / 32) a.label_logit[n0 + 32 * j + lane % 32] = logit;
+      }
+      float m = -INFINITY;
 #pragma unroll
       for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (v0 + 32 * i + acc_row(r, lane) >= a.g.a.rows) acc.c[i][j][r] = -INFINITY;
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, acc.c[i][j][r]);
+      m = fmaxf(top[j], __builtin_ceilf(m * kLog2e));
+      const float from = m == -INFINITY ? 0.0f : m;
+      float s = sum[j] * __builtin_amdgcn_exp2f(top[j] - from);
+#pragma unroll
+      for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][r], kLog2e, -from));
+      top[j] = m;
+      sum[j] = s;
     }
-    float m = -INFINITY;
+    clear(acc);
+  });
+  float2 *stats = reinterpret_cast<float2 *>(lds);  // [WM][BN]
 #pragma unroll
-    for (int i = 0; i < Tile::TM; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) m = fmaxf(m, acc.c[i][j][r]);
-    m = __builtin_ceilf(fmaxf(m, __shfl_xor(m, 32, kWaveSize)) * kLog2e);
-    const float from = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < Tile::TM; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][r], kLog2e, -from));
-    s += __shfl_xor(s, 32, kWaveSize);
-    if (lane < 32) stats[wm * Tile::BN + wn * (Tile::BN / Tile::WN) + 32 * j + lane] = float2{m, s};
+  for (int j = 0; j < Tile::TN; ++j) {
+    const float2 s = join_stats(float2{top[j], sum[j]},
+                                float2{__shfl_xor(top[j], 32, kWaveSize), __shfl_xor(sum[j], 32, kWaveSize)});
+    if (lane < 32) stats[wm * Tile::BN + wn * (Tile::BN / Tile::WN) + 32 * j + lane] = s;
   }
   __syncthreads();
   for (int c = threadIdx.x; c < Tile::BN; c += Tile::kThreads) {
@@ -263,53 +314,33 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
     float2 s = stats[c];
 #pragma unroll
     for (int w = 1; w < Tile::WM; ++w) s = join_stats(s, stats[w * Tile::BN + c]);
-    a.part[(static_cast<int64_t>(a.tile0) + at.tm) * a.g.b.rows + n] = s;
+    a.part[(static_cast<int64_t>(a.range0) + range) * a.g.b.rows + n] = s;
   }
 }
 
-// 16 rows per workgroup.  Its threads, 16 neighbouring ones per tile, share the tiles of vocabulary; then its waves take
-// the rows' labels, kVec elements per lane and step of the dot product.
+// 16 rows per workgroup, 16 threads per row share its ranges.  `loss` holds the label's logits on entry.
 constexpr int kLossRows = 16;
-template <typename T, typename Id, int kVec, int kThreads>
-__global__ __launch_bounds__(kThreads) void loss_kernel(const float2 *part, int32_t tiles, const T *h, const T *w,
-                                                        const Id *labels, int32_t N, int64_t V, int32_t D, float *loss,
-                                                        float *lse) {
-  constexpr int kShares = kThreads / kLossRows, kWaves = kThreads / kWaveSize;
+template <typename Id>
+__global__ __launch_bounds__(kBlockThreads) void loss_kernel(const float2 *part, int32_t ranges, const Id *labels,
+                                                             int32_t N, int64_t V, float *loss, float *lse) {
+  constexpr int kShares = kBlockThreads / kLossRows;
   __shared__ float2 joined[kShares][kLossRows];
-  __shared__ float row_lse[kLossRows];
   const int row = threadIdx.x % kLossRows, share = threadIdx.x / kLossRows;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kLossRows;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * kLossRows + row;
   float2 s{-INFINITY, 0.0f};
-  if (n0 + row < N)
-    for (int32_t t = share; t < tiles; t += kShares) s = join_stats(s, part[static_cast<int64_t>(t) * N + n0 + row]);
+  if (n < N)
+    for (int32_t t = share; t < ranges; t += kShares) s = join_stats(s, part[static_cast<int64_t>(t) * N + n]);
   joined[share][row] = s;
+#pragma unroll
   for (int half = kShares / 2; half > 0; half >>= 1) {
     __syncthreads();
     if (share < half) joined[share][row] = s = join_stats(s, joined[share + half][row]);
   }
-  if (share == 0) {
+  if (share == 0 && n < N) {
     const float r = static_cast<float>((static_cast<double>(s.x) + log2(static_cast<double>(s.y))) * 0.69314718055994530942);
-    row_lse[row] = r;
-    if (n0 + row < N) lse[n0 + row] = r;
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & (kWaveSize - 1);
-  for (int k = threadIdx.x / kWaveSize; k < kLossRows && n0 + k < N; k += kWaves) {
-    const Id y = labels[n0 + k];
-    const bool there = y >= 0 && static_cast<int64_t>(y) < V;
-    float dot = 0.0f;
-    if (there) {
-      using P = Pack<T, kVec>;
-      const T *a = h + (n0 + k) * D, *b = w + static_cast<int64_t>(y) * D;
-      for (int32_t c = lane * kVec; c < D; c += kWaveSize * kVec) {
-        const P pa = *reinterpret_cast<const P *>(a + c), pb = *reinterpret_cast<const P *>(b + c);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) dot = __builtin_fmaf(widen(pa.v[j]), widen(pb.v[j]), dot);
-      }
-#pragma unroll
-      for (int d = 1; d < kWaveSize; d <<= 1) dot += __shfl_xor(dot, d, kWaveSize);
-    }
-    if (lane == 0) loss[n0 + k] = there ? row_lse[k] - dot : 0.0f;
+    const Id y = labels[n];
+    lse[n] = r;
+    loss[n] = y >= 0 && static_cast<int64_t>(y) < V ? r - loss[n] : 0.0f;
   }
 }
 
@@ -375,18 +406,20 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
         acc.c[i][j][k] = label >= 0 ? p : 0.0f;
       }
     if (__any(hit >= 0 && hit < Tile::BM / Tile::WM)) {
+      const int mine = hit - acc_row(0, lane);
 #pragma unroll
       for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          if (32 * i + acc_row(k, lane) == hit) acc.c[i][j][k] -= times;
+          if (32 * i + acc_row(k, 0) == mine) acc.c[i][j][k] -= times;
     }
-    if (v0 + Tile::BM / Tile::WM > a.g.a.rows) {  // rows past the end are the last row again
+    if (v0 + Tile::BM / Tile::WM > a.g.a.rows) {  // nothing past the end
+      const int end = max(a.g.a.rows - v0, 0) - acc_row(0, lane);
 #pragma unroll
       for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          if (v0 + 32 * i + acc_row(k, lane) >= a.g.a.rows) acc.c[i][j][k] = 0.0f;
+          if (32 * i + acc_row(k, 0) >= end) acc.c[i][j][k] = 0.0f;
     }
   }
   constexpr int kPieces = Tile::BM / 8;  // of 16 bytes in a row of the [n, v] tile
@@ -493,7 +526,7 @@ __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
       return;
     }
   }
-  const int e = sizeof(T) == 4 ? -(kTop + exponent_for(*a.peak)) : 0;
+  const int e = sizeof(T) == 4 ? -(kTop + exponent_for(read_peak(a.peak))) : 0;
   float *part = kPartial ? a.part + at.split * a.part_stride : nullptr;
 #pragma unroll
   for (int i = 0; i < Tile::TM; ++i)
@@ -518,17 +551,41 @@ __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
     }
 }
 
-// out = sum over the splits, in order; rows with keep < 0 become zeros
-template <typename T>
+// out = sum over the splits; rows with keep < 0 become zeros.  Four elements per thread; kShares threads, one per wave,
+// share the splits where these are many and the elements few.
+template <typename T, int kShares>
 __global__ __launch_bounds__(kBlockThreads) void join_kernel(const float *part, int64_t part_stride, int32_t splits,
                                                              T *out, int64_t rows, int32_t D, const int32_t *keep) {
-  const int64_t total = rows * D, stride = static_cast<int64_t>(gridDim.x) * kBlockThreads;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x; t < total; t += stride) {
-    float s = 0.0f;
-    for (int32_t z = 0; z < splits; ++z) s += part[z * part_stride + t];
-    if (keep && keep[t / D] < 0) s = 0.0f;
-    out[t] = narrow<T>(s);
+  constexpr int kQuads = kBlockThreads / kShares;
+  __shared__ float4 joined[kShares][kQuads];
+  const int share = threadIdx.x / kQuads;
+  const int64_t total = rows * D, t = (static_cast<int64_t>(blockIdx.x) * kQuads + threadIdx.x % kQuads) * 4;
+  float4 s{0.0f, 0.0f, 0.0f, 0.0f};
+  if (t < total)
+    for (int32_t z = splits * share / kShares; z < splits * (share + 1) / kShares; ++z) {
+      const float4 x = *reinterpret_cast<const float4 *>(part + z * part_stride + t);
+      s.x += x.x;
+      s.y += x.y;
+      s.z += x.z;
+      s.w += x.w;
+    }
+  if constexpr (kShares > 1) {
+    joined[share][threadIdx.x % kQuads] = s;
+    __syncthreads();
+    if (share) return;
+#pragma unroll
+    for (int k = 1; k < kShares; ++k) {
+      const float4 x = joined[k][threadIdx.x];
+      s.x += x.x;
+      s.y += x.y;
+      s.z += x.z;
+      s.w += x.w;
+    }
   }
+  const float x[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (t + k < total) out[t + k] = narrow<T>(keep && keep[(t + k) / D] < 0 ? 0.0f : x[k]);
 }
 
 __global__ __launch_bounds__(kBlockThreads) void zero_kernel(uint16_t *out, int64_t n) {
@@ -540,9 +597,14 @@ __global__ __launch_bounds__(kBlockThreads) void zero_kernel(uint16_t *out, int6
 enum TileKind { kBig, kMid, kFlat, kTall };
 struct TileSize {
   int bm, bn, per_cu;
-  double rate;  // of the inner loop relative to the large tile
+  double step;                      // microseconds per step of k with every CU full
+  double stats, grad, store;        // ... per tile for the epilogues of the three kernels (16-bit results)
 };
-constexpr TileSize kTileSize[] = {{256, 256, 1, 1.0}, {128, 128, 2, 0.7}, {64, 256, 2, 0.6}, {256, 64, 2, 0.6}};
+// Measured on products of 1024 .. 8192 terms and epilogues of 4096 x 65536 logits.
+constexpr TileSize kTileSize[] = {{256, 256, 1, 1.95, 3.0, 15.0, 6.0},
+                                  {128, 128, 2, 1.15, 1.8, 9.0, 3.5},
+                                  {64, 256, 2, 1.25, 1.8, 9.0, 3.5},
+                                  {256, 64, 2, 1.25, 1.8, 9.0, 3.5}};
 constexpr int kCus = 256;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -551,34 +613,67 @@ int64_t steps_of(int64_t k) { return (k + kStepK - 1) / kStepK; }
 // at the same k do not all belong to the same few channels of the caches.
 int64_t pitch_of(int64_t k) { return (steps_of(k) | 1) * kStepK; }
 
-// The tile whose rounds of workgroups over the device take the least time; tiles that can share a long k among
-// several workgroups (`splittable`) are judged by their total work instead.
-TileKind choose_tile(int64_t M, int64_t N, bool splittable) {
+int64_t tiles_of(int64_t n, int64_t per) { return (n + per - 1) / per; }
+
+// Microseconds that `groups` workgroups of this kind take, each `work` with the device full.
+double rounds_time(const TileSize &s, int64_t groups, double work) {
+  const int64_t slots = kCus * s.per_cu;
+  if (groups <= kCus && s.per_cu > 1) return 0.7 * work;  // alone on its CU
+  return static_cast<double>((groups + slots - 1) / slots) * work;
+}
+
+// Ranges of the vocabulary tiles for the statistics: the division with the shortest time, each workgroup costing about
+// three microseconds to begin.
+constexpr int kMostRanges = 256;
+double choose_ranges(const TileSize &s, int64_t M, int64_t N, int64_t steps, int *ranges) {
+  const int64_t tiles_m = tiles_of(M, s.bm), tiles_n = tiles_of(N, s.bn);
+  double least = 0.0;
+  for (int64_t r = 1; r <= std::min<int64_t>(tiles_m, kMostRanges); ++r) {
+    const double t = rounds_time(s, tiles_n * r, static_cast<double>(tiles_of(tiles_m, r)) * (steps * s.step + s.stats) + 3.0);
+    if (r == 1 || t < least) {
+      *ranges = static_cast<int>(r);
+      least = t;
+    }
+  }
+  return least;
+}
+
+// Splits of a product's k: more workgroups where there are few tiles, against partial sums written and read again (about
+// 4 TB/s, and a launch).
+double choose_splits(const TileSize &s, int64_t M, int64_t N, int64_t steps, int *splits) {
+  const int64_t tiles = tiles_of(M, s.bm) * tiles_of(N, s.bn);
+  double least = 0.0;
+  for (int z = 1; z <= 256 && (z == 1 || (steps / z >= 4 && z * M * N <= (int64_t{1} << 28))); z += z < 8 ? 1 : z / 4) {
+    double t = rounds_time(s, tiles * z, static_cast<double>(tiles_of(steps, z)) * s.step + s.store);
+    if (z > 1) t += 4.0 + static_cast<double>(z) * M * N * 8.0 / 4e6;
+    if (z == 1 || t < least) {
+      *splits = z;
+      least = t;
+    }
+  }
+  return least;
+}
+
+// The kind of tile with the shortest time by `cost`.
+template <typename F>
+TileKind choose_tile(F &&cost) {
   if (const int forced = config().ce_tile) return static_cast<TileKind>(std::min(forced, 4) - 1);
   int best = kBig;
   double least = 0.0;
   for (int k = 0; k < 4; ++k) {
-    const TileSize &s = kTileSize[k];
-    const double tiles = static_cast<double>((M + s.bm - 1) / s.bm) * static_cast<double>((N + s.bn - 1) / s.bn);
-    const double rounds = splittable ? std::max(1.0, tiles / (kCus * s.per_cu)) : std::ceil(tiles / (kCus * s.per_cu));
-    const double cost = (splittable ? tiles / kCus : rounds * s.per_cu) * s.bm * s.bn / s.rate;
-    if (k == 0 || cost < least) {
+    const double t = cost(kTileSize[k]);
+    if (k == 0 || t < least) {
       best = k;
-      least = cost;
+      least = t;
     }
   }
   return static_cast<TileKind>(best);
 }
 
-// Workgroups per tile along k: enough to give every CU two, each with eight steps or more.
-int choose_splits(TileKind kind, int64_t M, int64_t N, int64_t steps) {
-  const TileSize &s = kTileSize[kind];
-  const int64_t tiles = ((M + s.bm - 1) / s.bm) * ((N + s.bn - 1) / s.bn);
-  const int64_t want = (kCus * s.per_cu + tiles - 1) / tiles;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(want, steps / 8)));
-}
-
-constexpr int64_t kPieceBytes = int64_t{512} << 20;  // copies and G of one piece of the vocabulary
+// Copies and P of one piece of the vocabulary.  As few pieces as memory allows: smaller ones, that the last-level cache
+// would hold, cost more in short launches than the cache gives back (4096 x 65536 x 1024: 2371 us for the gradient in
+// pieces of 256 MiB, 2005 of 512, 1891 of 1024, 1780 in one).
+constexpr int64_t kPieceBytes = int64_t{4} << 30;
 
 struct Layout {
   int parts, segments;
@@ -605,7 +700,6 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   if (const int64_t rows = config().ce_piece_rows) l.piece = up(rows, 256);
   const int64_t in_piece = std::min(l.piece, V), piece_p = pitch_of(in_piece);
   l.pieces = (V + l.piece - 1) / l.piece;
-  l.logits = choose_tile(in_piece, N, false);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -617,23 +711,30 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   if (dtype == FG_F32) {
     l.h_exp = take(4 * up(N, 256));
     l.w_exp = take(4 * up(in_piece, 256));
-    l.peaks = take(4 * (1 + l.pieces));
+    l.peaks = take(4 * kPeakSlots * kPeakStride * (1 + l.pieces));
   }
+  const int64_t steps = steps_of(D) * l.segments;
   if (!backward) {
-    const int64_t bm = kTileSize[l.logits].bm;
-    l.stats = take(l.pieces * ((l.piece + bm - 1) / bm) * N * 8);
+    int ranges;
+    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, &ranges); });
+    l.stats = take(l.pieces * std::min<int64_t>(tiles_of(l.piece, kTileSize[l.logits].bm), kMostRanges) * N * 8);
   } else {
-    l.dh = choose_tile(N, D, true);
-    l.dw = choose_tile(in_piece, D, true);
-    l.dh_splits = choose_splits(l.dh, N, D, steps_of(in_piece) * l.segments);
-    l.dw_splits = choose_splits(l.dw, in_piece, D, steps_of(N) * l.segments);
+    l.logits = choose_tile([&](const TileSize &s) {
+      return rounds_time(s, tiles_of(in_piece, s.bm) * tiles_of(N, s.bn), steps * s.step + l.parts * s.grad);
+    });
+    int z;
+    const int64_t dh_steps = steps_of(in_piece) * l.segments, dw_steps = steps_of(N) * l.segments;
+    l.dh = choose_tile([&](const TileSize &s) { return choose_splits(s, N, D, dh_steps, &z); });
+    l.dw = choose_tile([&](const TileSize &s) { return choose_splits(s, in_piece, D, dw_steps, &z); });
+    choose_splits(kTileSize[l.dh], N, D, dh_steps, &l.dh_splits);
+    choose_splits(kTileSize[l.dw], in_piece, D, dw_steps, &l.dw_splits);
     l.label = take(4 * N);
     l.ht = take(2 * l.parts * D * l.Np);
     l.wt = take(2 * l.parts * D * piece_p);
     l.nv = take(2 * l.parts * N * piece_p);
     l.vn = take(2 * l.parts * in_piece * l.Np);
-    l.dh_part = take(l.dh_splits > 1 || V > l.piece ? 4 * l.dh_splits * N * D : 0);
-    l.dw_part = take(l.dw_splits > 1 ? 4 * l.dw_splits * in_piece * D : 0);
+    l.dh_part = take(l.dh_splits > 1 || V > l.piece ? 4 * l.dh_splits * up(N * D, 4) : 0);
+    l.dw_part = take(l.dw_splits > 1 ? 4 * l.dw_splits * up(in_piece * D, 4) : 0);
   }
   l.bytes = std::max<int64_t>(at, 1024);
   return l;
@@ -699,10 +800,25 @@ void transpose(const T *x, const int32_t *keep, const float *factor, const uint3
                                                                      static_cast<int32_t>(D), pitch);
 }
 
+template <typename T>
+void join(const float *part, int64_t part_stride, int32_t splits, T *out, int64_t rows, int64_t D, const int32_t *keep,
+          hipStream_t stream) {
+  const int64_t quads = (rows * D + 3) / 4;
+  if (splits >= 16)
+    join_kernel<T, 8><<<dim3(static_cast<unsigned>((quads + 31) / 32)), dim3(kBlockThreads), 0, stream>>>(
+        part, part_stride, splits, out, rows, static_cast<int32_t>(D), keep);
+  else
+    join_kernel<T, 1><<<dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(kBlockThreads), 0, stream>>>(
+        part, part_stride, splits, out, rows, static_cast<int32_t>(D), keep);
+}
+
 template <typename T, typename Id>
 int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *labels, float *loss, float *lse,
             char *ws, const Layout &l, hipStream_t stream) {
   StatsArgs a{};
+  a.g.splits = 1;
+  a.labels = labels;
+  a.label_logit = loss;
   a.part = reinterpret_cast<float2 *>(ws + l.stats);
   a.g.steps = static_cast<int32_t>(steps_of(D));
   auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
@@ -711,25 +827,17 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
   a.g.b = operand(h, N, D, l, ws + l.h_pack, h_exp, nullptr, nullptr, nullptr, stream);
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
     a.g.a = operand(w + v0 * D, std::min(l.piece, V - v0), D, l, ws + l.w_pack, w_exp, nullptr, nullptr, nullptr, stream);
-    const int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3 grid) {
+    a.v0 = v0;
+    const int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3) {
       using Tile = decltype(tile);
-      stats_kernel<Tile, T><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
+      choose_ranges(kTileSize[l.logits], a.g.a.rows, N, steps_of(D) * l.segments, &a.ranges);
+      stats_kernel<Tile, T, Id><<<dim3(static_cast<unsigned>(a.ranges * a.g.tiles_n)), dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
-    a.tile0 += a.g.tiles_m;
+    a.range0 += a.ranges;
   }
-  const dim3 grid(static_cast<unsigned>((N + kLossRows - 1) / kLossRows));
-  auto join = [&](auto vec, auto threads) {
-    loss_kernel<T, Id, decltype(vec)::value, decltype(threads)::value><<<grid, dim3(threads.value), 0, stream>>>(
-        a.part, a.tile0, h, w, labels, static_cast<int32_t>(N), V, static_cast<int32_t>(D), loss, lse);
-  };
-  const bool wide = vector_elements(D, sizeof(T), {h, w}) >= 4;
-  using One = std::integral_constant<int, 1>;
-  using Four = std::integral_constant<int, 4>;
-  using Few = std::integral_constant<int, 256>;
-  using Many = std::integral_constant<int, 1024>;
-  if (a.tile0 > 64) wide ? join(Four{}, Many{}) : join(One{}, Many{});  // 64 threads per row, else 16
-  else wide ? join(Four{}, Few{}) : join(One{}, Few{});
+  loss_kernel<Id><<<dim3(static_cast<unsigned>((N + kLossRows - 1) / kLossRows)), dim3(kBlockThreads), 0, stream>>>(
+      a.part, a.range0, labels, static_cast<int32_t>(N), V, loss, lse);
   FG_HIP_TRY(hipGetLastError());
   return FG_OK;
 }
@@ -776,7 +884,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     a.pitch_v = static_cast<int32_t>(rows_p);
     a.nv_part = N * rows_p;
     a.vn_part = rows * l.Np;
-    uint32_t *peak = peaks ? peaks + 1 + v0 / l.piece : nullptr;
+    uint32_t *peak = peaks ? peaks + (1 + v0 / l.piece) * kPeakSlots * kPeakStride : nullptr;
     a.g.a = operand(w + v0 * D, rows, D, l, ws + l.w_pack, w_exp, peak, nullptr, nullptr, stream);
     int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3 grid) {
       using Tile = decltype(tile);
@@ -792,12 +900,11 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     s.g.b = GemmOperand{ht, D * l.Np, l.Np, static_cast<int32_t>(D)};
     s.peak = peaks;
     s.part = reinterpret_cast<float *>(ws + l.dw_part);
-    s.part_stride = rows * D;
+    s.part_stride = up(rows * D, 4);
     rc = product<T>(l.dw, s, dw + v0 * D, l.dw_splits > 1, stream);
     if (rc) return rc;
     if (l.dw_splits > 1)
-      join_kernel<T><<<dim3(flat_grid(rows * D)), dim3(kBlockThreads), 0, stream>>>(
-          s.part, s.part_stride, l.dw_splits, dw + v0 * D, rows, static_cast<int32_t>(D), nullptr);
+      join<T>(s.part, s.part_stride, l.dw_splits, dw + v0 * D, rows, D, nullptr, stream);
 
     s.g.steps = static_cast<int32_t>(steps_of(rows));  // dh[n, d] = sum over v of G[n, v] * w[v, d]
     s.g.splits = l.dh_splits;
@@ -807,14 +914,13 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     s.factor = factor;
     s.peak = peak;
     s.part = reinterpret_cast<float *>(ws + l.dh_part);
-    s.part_stride = N * D;
+    s.part_stride = up(N * D, 4);
     s.accumulate = v0 > 0;
     rc = product<T>(l.dh, s, dh, dh_partial, stream);
     if (rc) return rc;
   }
   if (dh_partial)
-    join_kernel<T><<<dim3(flat_grid(N * D)), dim3(kBlockThreads), 0, stream>>>(
-        reinterpret_cast<float *>(ws + l.dh_part), N * D, l.dh_splits, dh, N, static_cast<int32_t>(D), label);
+    join<T>(reinterpret_cast<float *>(ws + l.dh_part), up(N * D, 4), l.dh_splits, dh, N, D, label, stream);
   FG_HIP_TRY(hipGetLastError());
   return FG_OK;
 }
@@ -894,7 +1000,7 @@ int fg_linear_ce_grad(int64_t N, int64_t V, int64_t D, const void *hidden, const
   char *ws = static_cast<char *>(workspace);
   int32_t *label = reinterpret_cast<int32_t *>(ws + l.label);
   uint32_t *peaks = reinterpret_cast<uint32_t *>(ws + l.peaks);
-  const int32_t n_peaks = dtype == FG_F32 ? static_cast<int32_t>(1 + l.pieces) : 0;
+  const int32_t n_peaks = dtype == FG_F32 ? static_cast<int32_t>(fg::kPeakSlots * fg::kPeakStride * (1 + l.pieces)) : 0;
   const dim3 grid(static_cast<unsigned>((N + fg::kBlockThreads - 1) / fg::kBlockThreads));
   if (itype == FG_I32)
     fg::labels_kernel<int32_t><<<grid, dim3(fg::kBlockThreads), 0, s>>>(static_cast<const int32_t *>(labels), static_cast<int32_t>(N), V, label, peaks, n_peaks);

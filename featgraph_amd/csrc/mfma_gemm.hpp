@@ -125,8 +125,21 @@ __device__ __forceinline__ void arrive_and_meet() {
 #endif
 }
 
-template <typename Tile, typename T>
-__device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &at, uint16_t *lds, GemmAcc<Tile> &acc) {
+// The tiles at.tm .. at.tm + tiles - 1 of m one after the other, as one sequence of loads: done(i) is called with the sums
+// of the i-th in acc while the next one's first rows are under way to LDS, and zeroes acc with clear() if more follow.
+template <typename Tile>
+__device__ __forceinline__ void clear(GemmAcc<Tile> &acc) {
+#pragma unroll
+  for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < Tile::TN; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc.c[i][j][r] = 0.0f;
+}
+
+template <typename Tile, typename T, typename Done>
+__device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &at, int tiles, uint16_t *lds,
+                                           GemmAcc<Tile> &acc, Done &&done) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass lacks the loads to LDS
   using LdsPtr = __attribute__((address_space(3))) void *;
   using M = Multiply<T>;
@@ -134,53 +147,55 @@ __device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &a
   const int lane = threadIdx.x & (kWaveSize - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
-#pragma unroll
-  for (int i = 0; i < Tile::TM; ++i)
-#pragma unroll
-    for (int j = 0; j < Tile::TN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc.c[i][j][r] = 0.0f;
+  clear(acc);
 
   // what this lane fetches: row lane / 8 of the eight of a load, the piece that belongs at place lane % 8
   const int64_t m0 = static_cast<int64_t>(at.tm) * Tile::BM, n0 = static_cast<int64_t>(at.tn) * Tile::BN;
-  const int rows_a = static_cast<int>(min<int64_t>(Tile::BM, g.a.rows - m0));
-  const int rows_b = static_cast<int>(min<int64_t>(Tile::BN, g.b.rows - n0));
   const uint32_t pitch_a = static_cast<uint32_t>(g.a.pitch) * 2, pitch_b = static_cast<uint32_t>(g.b.pitch) * 2;
   uint32_t off_a[Tile::kLoadsA], off_b[Tile::kLoadsB];
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsA; ++j) {
     const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
-    off_a[j] = min(row, rows_a - 1) * pitch_a + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
+    off_a[j] = row * pitch_a + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
   }
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsB; ++j) {
     const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
-    off_b[j] = min(row, rows_b - 1) * pitch_b + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
+    off_b[j] = row * pitch_b + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
   }
-  const uint32_t bytes_a = rows_a * pitch_a, bytes_b = rows_b * pitch_b;
+  const uint32_t bytes_b = static_cast<uint32_t>(min<int64_t>(Tile::BN, g.b.rows - n0)) * pitch_b;
 
   const int total = g.steps * M::kSegments;
   const int first = static_cast<int>(static_cast<int64_t>(total) * at.split / g.splits);
   const int last = static_cast<int>(static_cast<int64_t>(total) * (at.split + 1) / g.splits);
-  // Loads of one step of an operand: its parts (segment 0 is hi * lo, 1 is lo * hi, 2 or the only one hi * hi), its k and
-  // its stage.  Past the last step nothing is fetched (no bytes are in range), so that the loop has no branches around
-  // its loads and always the same number of them under way.
+  const int per_tile = last - first, n = per_tile * tiles;
+  // Loads of one step of an operand: its parts (segment 0 is hi * lo, 1 is lo * hi, 2 or the only one hi * hi), its k, its
+  // tile and its stage.  Past the last step nothing is fetched (no bytes are in range), so that the loop has no branches
+  // around its loads and always the same number of them under way.
   struct Cursor {
-    int seg, step, slot, left;
+    int seg, step, slot, left, tile_left;
+    int64_t m;
   };
-  const int n = last - first;
-  Cursor ca{first / g.steps, first % g.steps, 0, n}, cb = ca;
+  const int first_seg = first / g.steps, first_step = first - first_seg * g.steps;
+  Cursor ca{first_seg, first_step, 0, n, per_tile, m0}, cb = ca;
   auto advance = [&](Cursor &c, int stages) {
     --c.left;
     if (++c.step == g.steps) {
       c.step = 0;
       ++c.seg;
     }
+    if (--c.tile_left == 0) {
+      c.tile_left = per_tile;
+      c.seg = first_seg;
+      c.step = first_step;
+      c.m += Tile::BM;
+    }
     if (++c.slot == stages) c.slot = 0;
   };
   uint16_t *const lds_b = lds + Tile::kStagesA * Tile::kStageA;
   auto load_a = [&](int j) {
-    const uint16_t *p = g.a.p + (M::kSegments == 3 && ca.seg == 1 ? g.a.part : 0) + m0 * g.a.pitch;
+    const uint16_t *p = g.a.p + (M::kSegments == 3 && ca.seg == 1 ? g.a.part : 0) + ca.m * g.a.pitch;
+    const uint32_t bytes_a = static_cast<uint32_t>(min<int64_t>(Tile::BM, g.a.rows - ca.m)) * pitch_a;
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, ca.left > 0 ? bytes_a : 0, 0x00020000);
     uint16_t *to = lds + ca.slot * Tile::kStageA + (wave + j * Tile::kWaves) * 8 * kStepK;
@@ -266,8 +281,9 @@ __device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &a
   for (int l = 0; l < kPerQuarter; ++l) load_one(l);
   arrive_and_meet<kPerQuarter + (kDeep ? Tile::kLoadsA : 0)>();
   read(f0, 0);
-  for (int i = 0; i < n; ++i) {
-    if (M::kSegments == 3 && i > 0 && i == cross) lower();
+  int tile = 0;
+  for (int i = 0, in_tile = 0; i < n; ++i) {
+    if (M::kSegments == 3 && in_tile > 0 && in_tile == cross) lower();
     read(f1, 1);
     multiply(f0, Q1{});
     read(f0, 2);
@@ -280,10 +296,21 @@ __device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &a
     slot_b ^= 1;
     read(f0, 0);  // past the last step: what is read is not used
     multiply(f1, Q0{});
+    if (++in_tile == per_tile) {
+      if (M::kSegments == 3 && cross >= per_tile) lower();
+      done(tile);
+      in_tile = 0;
+      ++tile;
+    }
   }
-  if (M::kSegments == 3 && cross >= n) lower();
-  arrive_and_meet<0>();  // the epilogue may use the LDS
+  arrive_and_meet<0>();  // the LDS may be used for other things
 #endif
+}
+
+// One tile, left in acc.
+template <typename Tile, typename T>
+__device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &at, uint16_t *lds, GemmAcc<Tile> &acc) {
+  gemm_tiles<Tile, T>(g, at, 1, lds, acc, [](int) {});
 }
 
 }  // namespace fg
