@@ -10,7 +10,7 @@
 // own.  Backward: the logits are computed again piece by piece of the vocabulary; the epilogue turns them into P,
 // written once as [n, v] and once as [v, n], and two more products over them give the piece's rows of dw and its
 // share of dh.  All three products are the same kernel over operands with k contiguous, so h and w are transposed
-// into padded copies for the backward products (2 N D + 2 V D elements of traffic against 6 N V D flops).
+// into copies for the backward products (2 N D + 2 V D elements of traffic against 6 N V D flops).
 //
 // Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step of each
 // term, random in sign; the results are rounded to bfloat16 themselves); everything between is float32.  float32
@@ -82,24 +82,24 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
   return u < 0x7f800000u ? u : 0u;
 }
 
-// bfloat16: [rows, D] -> [rows, Dp], zeros behind D
-__global__ __launch_bounds__(kBlockThreads) void pad_kernel(const uint16_t *x, uint16_t *out, int64_t rows, int32_t D,
-                                                            int32_t Dp) {
-  const int64_t total = rows * Dp, stride = static_cast<int64_t>(gridDim.x) * kBlockThreads;
+// bfloat16: [rows, D] -> panels
+__global__ __launch_bounds__(kBlockThreads) void pad_kernel(const uint16_t *x, uint16_t *out, int64_t rows, int32_t D) {
+  const int64_t total = rows * ((D + kStepK - 1) / kStepK * kStepK), stride = static_cast<int64_t>(gridDim.x) * kBlockThreads;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x; t < total; t += stride) {
-    const int64_t r = t / Dp;
-    const int32_t c = static_cast<int32_t>(t - r * Dp);
-    out[t] = c < D ? x[r * D + c] : 0;
+    const int64_t panel = t / (rows * kStepK), in_panel = t - panel * (rows * kStepK);
+    const int64_t c = panel * kStepK + in_panel % kStepK;
+    out[t] = c < D ? x[in_panel / kStepK * D + c] : 0;
   }
 }
 
-// float32: [rows, D] -> two parts of [rows, Dp], zeros behind D, each row by its own exponent (exps).  One wave per row.
+// float32: [rows, D] -> two parts as panels, each row by its own exponent (exps).  One wave per row.
 // peak (or null): largest |x| * |factor[row]| over the rows whose keep[] is not negative, for the transposed copy.
 __global__ __launch_bounds__(kBlockThreads) void split_rows_kernel(const float *x, uint16_t *out, int64_t rows,
-                                                                   int32_t D, int32_t Dp, int32_t *exps, uint32_t *peak,
+                                                                   int32_t D, int32_t *exps, uint32_t *peak,
                                                                    const int32_t *keep, const float *factor) {
   __shared__ uint32_t peaks[kWavesPerBlock];
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
+  const int32_t Dp = (D + kStepK - 1) / kStepK * kStepK;
   const int64_t part = rows * Dp, stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
   uint32_t most = 0;
   for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave; r < rows; r += stride) {
@@ -112,8 +112,9 @@ __global__ __launch_bounds__(kBlockThreads) void split_rows_kernel(const float *
     if (lane == 0) exps[r] = e;
     for (int32_t c = lane; c < Dp; c += kWaveSize) {
       const float y = c < D ? __builtin_ldexpf(row[c], e) : 0.0f;
-      out[r * Dp + c] = static_cast<uint16_t>(part_of<float>(y, 0));
-      out[part + r * Dp + c] = static_cast<uint16_t>(part_of<float>(y, 1));
+      const int64_t to = panel_at(rows, r, c);
+      out[to] = static_cast<uint16_t>(part_of<float>(y, 0));
+      out[part + to] = static_cast<uint16_t>(part_of<float>(y, 1));
     }
     if (peak && (!keep || keep[r] >= 0))
       most = max(most, finite_bits(__builtin_bit_cast(float, top) * (factor ? factor[r] : 1.0f)));
@@ -127,13 +128,13 @@ __global__ __launch_bounds__(kBlockThreads) void split_rows_kernel(const float *
   }
 }
 
-// [rows, D] -> parts of [D, pitch], zeros behind the rows and in place of rows whose keep[] is negative (whatever those
+// [rows, D] -> parts of its transpose as panels of 64 rows' elements, zeros in place of rows whose keep[] is negative (whatever those
 // hold must not reach the sum over rows).  float32: times factor[row] (or 1) and brought into range by *peak.
 // 64 x 64 elements per workgroup, 16 bytes per lane on both sides where D allows (kVec elements per load).
 template <typename T, int kVec>
 __global__ __launch_bounds__(kBlockThreads) void transpose_kernel(const T *x, const int32_t *keep, const float *factor,
                                                                   const uint32_t *peak, uint16_t *out, int32_t rows,
-                                                                  int32_t D, int64_t pitch) {
+                                                                  int32_t D) {
   constexpr int kLanes = 64 / kVec;  // per row
   __shared__ float tile[64][65];
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
@@ -156,14 +157,14 @@ __global__ __launch_bounds__(kBlockThreads) void transpose_kernel(const T *x, co
   __syncthreads();
   for (int t = threadIdx.x; t < 512; t += kBlockThreads) {  // eight rows of one column each
     const int g = t % 8, col = t / 8;
-    const int64_t r = r0 + 8 * g;
-    if (c0 + col >= D || r >= pitch) continue;
+    if (c0 + col >= D) continue;
 #pragma unroll
     for (int p = 0; p < Multiply<T>::kParts; ++p) {
       Pack<uint16_t, 8> y;
 #pragma unroll
       for (int k = 0; k < 8; ++k) y.v[k] = static_cast<uint16_t>(part_of<T>(tile[8 * g + k][col], p));
-      *reinterpret_cast<Pack<uint16_t, 8> *>(out + p * D * pitch + static_cast<int64_t>(c0 + col) * pitch + r) = y;
+      const int64_t panel = blockIdx.x + static_cast<int64_t>(p) * gridDim.x;  // a part has gridDim.x panels
+      *reinterpret_cast<Pack<uint16_t, 8> *>(out + (panel * D + c0 + col) * kStepK + 8 * g) = y;
     }
   }
 }
@@ -238,12 +239,10 @@ template <typename Tile, typename T, typename Id>
 __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
-  const uint32_t die = blockIdx.x % kXcds, q = gridDim.x / kXcds;  // consecutive ids on one die, as in gemm_place
-  const uint32_t id = die * q + min<uint32_t>(die, gridDim.x % kXcds) + blockIdx.x / kXcds;
-  const int range = static_cast<int>(id / a.g.tiles_n);
-  GemmPlace at;
-  at.split = 0;
-  at.tn = static_cast<int32_t>(id - static_cast<uint32_t>(range) * a.g.tiles_n);
+  GemmShape places = a.g;
+  places.tiles_m = a.ranges;
+  GemmPlace at = gemm_place(places);
+  const int range = at.tm;
   at.tm = static_cast<int32_t>(static_cast<int64_t>(a.g.tiles_m) * range / a.ranges);
   const int tiles = static_cast<int>(static_cast<int64_t>(a.g.tiles_m) * (range + 1) / a.ranges) - at.tm;
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
@@ -367,9 +366,8 @@ struct GradArgs {
   const int32_t *label;      // [N], negative: ignored
   const float *lse, *dloss;  // [N]
   int32_t v0;                // first vocabulary row of the piece
-  uint16_t *nv, *vn;         // P as [N, pitch_v] and [rows of the piece, pitch_n], parts apart by *_part
+  uint16_t *nv, *vn;         // P as panels of [n, v] and of [v, n], parts apart by *_part
   int64_t nv_part, vn_part;
-  int32_t pitch_v, pitch_n;  // multiples of 64; what is behind the ends is written as zeros
 };
 
 // T: type of the operands, which says how P is stored.  The [v, n] copy is written from the registers, four n per lane;
@@ -435,7 +433,9 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
   };
   const int64_t first_n = static_cast<int64_t>(at.tn) * Tile::BN;
   const int first_v = at.tm * Tile::BM;
-  const bool whole = first_v + Tile::BM <= a.g.a.rows && first_n + Tile::BN <= a.g.b.rows;
+  const int64_t M = a.g.a.rows, N = a.g.b.rows;
+  const int64_t end_v = (M + kStepK - 1) / kStepK * kStepK, end_n = (N + kStepK - 1) / kStepK * kStepK;  // of the panels
+  const bool whole = first_v + Tile::BM <= M && first_n + Tile::BN <= N;
   auto store = [&](auto inside, int part) {  // inside: the whole tile lies within the matrix
     constexpr bool kInside = decltype(inside)::value;
 #pragma unroll
@@ -445,7 +445,8 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
 #pragma unroll
       for (int i = 0; i < Tile::TM; ++i) {
         FG_IN_ORDER();
-        uint16_t *to = a.vn + part * a.vn_part + static_cast<int64_t>(v0 + 32 * i + acc_row(0, lane) + lane % 4) * a.pitch_n + col;
+        const int64_t row = v0 + 32 * i + acc_row(0, lane) + lane % 4;
+        uint16_t *to = a.vn + part * a.vn_part + panel_at(M, row, col);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float e[4] = {acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
@@ -459,17 +460,16 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
           const int v = wave_v + 32 * i + 8 * q;  // lanes 32..63: the second half of the piece
           *reinterpret_cast<uint2 *>(lds + n * Tile::BM + place(n, v / 8) * 8 + lane / 32 * 4) = x;
           const uint2 y = turn4(x, lane);
-          if (kInside || (v0 + 32 * i + acc_row(4 * q, lane) + lane % 4 < a.g.a.rows && col < a.pitch_n))
-            *reinterpret_cast<uint2 *>(to + static_cast<int64_t>(8 * q) * a.pitch_n) = y;
+          if (kInside || (row + 8 * q < M && col < end_n)) *reinterpret_cast<uint2 *>(to + 8 * q * kStepK) = y;
         }
       }
     }
     __syncthreads();
 #pragma unroll 4
-    for (int t = threadIdx.x; t < Tile::BN * kPieces; t += Tile::kThreads) {
-      const int n = t / kPieces, piece = t % kPieces;
-      if (kInside || (first_n + n < a.g.b.rows && first_v + piece * 8 < a.pitch_v))
-        *reinterpret_cast<uint4 *>(a.nv + part * a.nv_part + (first_n + n) * a.pitch_v + first_v + piece * 8) =
+    for (int t = threadIdx.x; t < Tile::BN * kPieces; t += Tile::kThreads) {  // panel by panel, eight pieces per row
+      const int piece = t / (8 * Tile::BN) * 8 + t % 8, n = t / 8 % Tile::BN;
+      if (kInside || (first_n + n < N && first_v + piece * 8 < end_v))
+        *reinterpret_cast<uint4 *>(a.nv + part * a.nv_part + panel_at(N, first_n + n, first_v + piece * 8)) =
             *reinterpret_cast<const uint4 *>(lds + n * Tile::BM + place(n, piece) * 8);
     }
   };
@@ -609,9 +609,6 @@ constexpr int kCus = 256;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t steps_of(int64_t k) { return (k + kStepK - 1) / kStepK; }
-// Elements from one row of a copy to the next: an odd number of 128-byte lines, so that the lines which a tile's rows need
-// at the same k do not all belong to the same few channels of the caches.
-int64_t pitch_of(int64_t k) { return (steps_of(k) | 1) * kStepK; }
 
 int64_t tiles_of(int64_t n, int64_t per) { return (n + per - 1) / per; }
 
@@ -679,7 +676,6 @@ struct Layout {
   int parts, segments;
   int64_t pieces;
   bool packed;           // operands copied with k padded (float32, or rows that are no multiple of kStepK or 16 bytes)
-  int64_t Dp, Np;        // pitches of rows of D and N elements
   int64_t piece;         // vocabulary rows per piece, a multiple of 256
   TileKind logits, dh, dw;
   int dh_splits, dw_splits;
@@ -691,14 +687,12 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   l.parts = dtype == FG_F32 ? kParts : 1;
   l.segments = dtype == FG_F32 ? kSegments : 1;
   l.packed = dtype == FG_F32 || D % kStepK != 0 || !aligned;
-  l.Dp = pitch_of(D);
-  l.Np = pitch_of(N);
-  int64_t per_row = l.packed ? 2 * l.parts * l.Dp : 0;
-  if (backward) per_row += 2 * l.parts * (2 * l.Np + D);
+  int64_t per_row = l.packed ? 2 * l.parts * up(D, kStepK) : 0;
+  if (backward) per_row += 2 * l.parts * (N + up(N, kStepK) + D);
   const int64_t most = per_row ? std::max<int64_t>(256, kPieceBytes / per_row / 256 * 256) : up(V, 256);
   l.piece = up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), 256);  // as many pieces as needed, of equal size
   if (const int64_t rows = config().ce_piece_rows) l.piece = up(rows, 256);
-  const int64_t in_piece = std::min(l.piece, V), piece_p = pitch_of(in_piece);
+  const int64_t in_piece = std::min(l.piece, V);
   l.pieces = (V + l.piece - 1) / l.piece;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -706,8 +700,8 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
     at += up(bytes, 1024);
     return here;
   };
-  l.h_pack = take(l.packed ? 2 * l.parts * N * l.Dp : 0);
-  l.w_pack = take(l.packed ? 2 * l.parts * in_piece * l.Dp : 0);
+  l.h_pack = take(l.packed ? 2 * l.parts * panel_elements(N, D) : 0);
+  l.w_pack = take(l.packed ? 2 * l.parts * panel_elements(in_piece, D) : 0);
   if (dtype == FG_F32) {
     l.h_exp = take(4 * up(N, 256));
     l.w_exp = take(4 * up(in_piece, 256));
@@ -729,10 +723,10 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
     choose_splits(kTileSize[l.dh], N, D, dh_steps, &l.dh_splits);
     choose_splits(kTileSize[l.dw], in_piece, D, dw_steps, &l.dw_splits);
     l.label = take(4 * N);
-    l.ht = take(2 * l.parts * D * l.Np);
-    l.wt = take(2 * l.parts * D * piece_p);
-    l.nv = take(2 * l.parts * N * piece_p);
-    l.vn = take(2 * l.parts * in_piece * l.Np);
+    l.ht = take(2 * l.parts * panel_elements(D, N));
+    l.wt = take(2 * l.parts * panel_elements(D, in_piece));
+    l.nv = take(2 * l.parts * panel_elements(N, in_piece));
+    l.vn = take(2 * l.parts * panel_elements(in_piece, N));
     l.dh_part = take(l.dh_splits > 1 || V > l.piece ? 4 * l.dh_splits * up(N * D, 4) : 0);
     l.dw_part = take(l.dw_splits > 1 ? 4 * l.dw_splits * up(in_piece * D, 4) : 0);
   }
@@ -766,38 +760,35 @@ unsigned flat_grid(int64_t threads) {
 template <typename T>
 GemmOperand operand(const T *x, int64_t rows, int64_t D, const Layout &l, char *copy, int32_t *exps, uint32_t *peak,
                     const int32_t *keep, const float *factor, hipStream_t stream) {
-  GemmOperand o;
-  o.rows = static_cast<int32_t>(rows);
   if (!l.packed) {
+    GemmOperand o;
+    o.rows = static_cast<int32_t>(rows);
     o.p = reinterpret_cast<const uint16_t *>(x);
-    o.pitch = D;
+    o.row = D;
+    o.step = kStepK;
     return o;
   }
   auto *to = reinterpret_cast<uint16_t *>(copy);
   if constexpr (sizeof(T) == 4)
     split_rows_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>((rows + kWavesPerBlock - 1) / kWavesPerBlock, 4096))),
-                        dim3(kBlockThreads), 0, stream>>>(x, to, rows, static_cast<int32_t>(D),
-                                                          static_cast<int32_t>(l.Dp), exps, peak, keep, factor);
+                        dim3(kBlockThreads), 0, stream>>>(x, to, rows, static_cast<int32_t>(D), exps, peak, keep, factor);
   else
-    pad_kernel<<<dim3(flat_grid(rows * l.Dp)), dim3(kBlockThreads), 0, stream>>>(
-        reinterpret_cast<const uint16_t *>(x), to, rows, static_cast<int32_t>(D), static_cast<int32_t>(l.Dp));
-  o.p = to;
-  o.part = rows * l.Dp;
-  o.pitch = l.Dp;
-  return o;
+    pad_kernel<<<dim3(flat_grid(panel_elements(rows, D))), dim3(kBlockThreads), 0, stream>>>(
+        reinterpret_cast<const uint16_t *>(x), to, rows, static_cast<int32_t>(D));
+  return panels(to, rows, D);
 }
 
 template <typename T>
 void transpose(const T *x, const int32_t *keep, const float *factor, const uint32_t *peak, uint16_t *out, int64_t rows,
-               int64_t D, int64_t pitch, hipStream_t stream) {
+               int64_t D, hipStream_t stream) {
   constexpr int kVec = 16 / sizeof(T);
-  const dim3 grid(static_cast<unsigned>((pitch + 63) / 64), static_cast<unsigned>((D + 63) / 64));
+  const dim3 grid(static_cast<unsigned>(steps_of(rows)), static_cast<unsigned>((D + 63) / 64));
   if (D % kVec == 0 && aligned_to(x, 16))
     transpose_kernel<T, kVec><<<grid, dim3(kBlockThreads), 0, stream>>>(x, keep, factor, peak, out, static_cast<int32_t>(rows),
-                                                                        static_cast<int32_t>(D), pitch);
+                                                                        static_cast<int32_t>(D));
   else
     transpose_kernel<T, 1><<<grid, dim3(kBlockThreads), 0, stream>>>(x, keep, factor, peak, out, static_cast<int32_t>(rows),
-                                                                     static_cast<int32_t>(D), pitch);
+                                                                     static_cast<int32_t>(D));
 }
 
 template <typename T>
@@ -868,7 +859,6 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   a.dloss = dloss;
   a.nv = nv;
   a.vn = vn;
-  a.pitch_n = static_cast<int32_t>(l.Np);
   a.g.steps = static_cast<int32_t>(steps_of(D));
   auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
   uint32_t *peaks = sizeof(T) == 4 ? reinterpret_cast<uint32_t *>(ws + l.peaks) : nullptr;  // of h, then of each piece of w
@@ -876,14 +866,13 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   a.exp_a = w_exp;
   a.exp_b = h_exp;
   a.g.b = operand(h, N, D, l, ws + l.h_pack, h_exp, peaks, label, factor, stream);
-  transpose(h, label, factor, peaks, ht, N, D, l.Np, stream);
+  transpose(h, label, factor, peaks, ht, N, D, stream);
   const bool dh_partial = l.dh_splits > 1 || V > l.piece;
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
-    const int64_t rows = std::min(l.piece, V - v0), rows_p = pitch_of(rows);
+    const int64_t rows = std::min(l.piece, V - v0);
     a.v0 = static_cast<int32_t>(v0);
-    a.pitch_v = static_cast<int32_t>(rows_p);
-    a.nv_part = N * rows_p;
-    a.vn_part = rows * l.Np;
+    a.nv_part = panel_elements(N, rows);
+    a.vn_part = panel_elements(rows, N);
     uint32_t *peak = peaks ? peaks + (1 + v0 / l.piece) * kPeakSlots * kPeakStride : nullptr;
     a.g.a = operand(w + v0 * D, rows, D, l, ws + l.w_pack, w_exp, peak, nullptr, nullptr, stream);
     int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3 grid) {
@@ -891,13 +880,13 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
       grad_logits_kernel<Tile, T><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
-    transpose<T>(w + v0 * D, nullptr, nullptr, peak, wt, rows, D, rows_p, stream);
+    transpose<T>(w + v0 * D, nullptr, nullptr, peak, wt, rows, D, stream);
 
     StoreArgs s{};  // dw[v, d] = sum over n of G[v, n] * h[n, d]
     s.g.steps = static_cast<int32_t>(steps_of(N));
     s.g.splits = l.dw_splits;
-    s.g.a = GemmOperand{vn, a.vn_part, l.Np, static_cast<int32_t>(rows)};
-    s.g.b = GemmOperand{ht, D * l.Np, l.Np, static_cast<int32_t>(D)};
+    s.g.a = panels(vn, rows, N);
+    s.g.b = panels(ht, D, N);
     s.peak = peaks;
     s.part = reinterpret_cast<float *>(ws + l.dw_part);
     s.part_stride = up(rows * D, 4);
@@ -908,8 +897,8 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
 
     s.g.steps = static_cast<int32_t>(steps_of(rows));  // dh[n, d] = sum over v of G[n, v] * w[v, d]
     s.g.splits = l.dh_splits;
-    s.g.a = GemmOperand{nv, a.nv_part, rows_p, static_cast<int32_t>(N)};
-    s.g.b = GemmOperand{wt, D * rows_p, rows_p, static_cast<int32_t>(D)};
+    s.g.a = panels(nv, N, rows);
+    s.g.b = panels(wt, D, rows);
     s.keep = label;
     s.factor = factor;
     s.peak = peak;

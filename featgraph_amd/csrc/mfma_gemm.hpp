@@ -62,9 +62,24 @@ struct Multiply<float> {
 struct GemmOperand {
   const uint16_t *p = nullptr;  // part 0
   int64_t part = 0;             // elements from one part to the next
-  int64_t pitch = 0;            // elements from one row to the next, a multiple of 8
+  int64_t row = kStepK;         // elements from one row to the next, a multiple of 8
+  int64_t step = 0;             // elements from one step of k to the next
   int32_t rows = 0;
 };
+
+// Parts of `rows` rows of k elements each, as panels.
+inline int64_t panel_elements(int64_t rows, int64_t k) { return (k + kStepK - 1) / kStepK * kStepK * rows; }
+inline GemmOperand panels(const uint16_t *p, int64_t rows, int64_t k) {
+  GemmOperand o;
+  o.p = p;
+  o.part = panel_elements(rows, k);
+  o.step = rows * kStepK;
+  o.rows = static_cast<int32_t>(rows);
+  return o;
+}
+__device__ __forceinline__ int64_t panel_at(int64_t rows, int64_t row, int64_t k) {
+  return k / kStepK * (rows * kStepK) + row * kStepK + k % kStepK;
+}
 
 struct GemmShape {
   GemmOperand a, b;
@@ -151,7 +166,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
 
   // what this lane fetches: row lane / 8 of the eight of a load, the piece that belongs at place lane % 8
   const int64_t m0 = static_cast<int64_t>(at.tm) * Tile::BM, n0 = static_cast<int64_t>(at.tn) * Tile::BN;
-  const uint32_t pitch_a = static_cast<uint32_t>(g.a.pitch) * 2, pitch_b = static_cast<uint32_t>(g.b.pitch) * 2;
+  const uint32_t pitch_a = static_cast<uint32_t>(g.a.row) * 2, pitch_b = static_cast<uint32_t>(g.b.row) * 2;
   uint32_t off_a[Tile::kLoadsA], off_b[Tile::kLoadsB];
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsA; ++j) {
@@ -163,7 +178,8 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
     off_b[j] = row * pitch_b + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
   }
-  const uint32_t bytes_b = static_cast<uint32_t>(min<int64_t>(Tile::BN, g.b.rows - n0)) * pitch_b;
+  // bytes in range: the rows that are there, of each the line of this step
+  const uint32_t bytes_b = static_cast<uint32_t>(min<int64_t>(Tile::BN, g.b.rows - n0) - 1) * pitch_b + kStepK * 2;
 
   const int total = g.steps * M::kSegments;
   const int first = static_cast<int>(static_cast<int64_t>(total) * at.split / g.splits);
@@ -194,19 +210,19 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
   };
   uint16_t *const lds_b = lds + Tile::kStagesA * Tile::kStageA;
   auto load_a = [&](int j) {
-    const uint16_t *p = g.a.p + (M::kSegments == 3 && ca.seg == 1 ? g.a.part : 0) + ca.m * g.a.pitch;
-    const uint32_t bytes_a = static_cast<uint32_t>(min<int64_t>(Tile::BM, g.a.rows - ca.m)) * pitch_a;
+    const uint16_t *p = g.a.p + (M::kSegments == 3 && ca.seg == 1 ? g.a.part : 0) + ca.m * g.a.row + ca.step * g.a.step;
+    const uint32_t bytes_a = static_cast<uint32_t>(min<int64_t>(Tile::BM, g.a.rows - ca.m) - 1) * pitch_a + kStepK * 2;
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, ca.left > 0 ? bytes_a : 0, 0x00020000);
     uint16_t *to = lds + ca.slot * Tile::kStageA + (wave + j * Tile::kWaves) * 8 * kStepK;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_a[j], ca.step * (kStepK * 2), 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_a[j], 0, 0, 0);
   };
   auto load_b = [&](int j) {
-    const uint16_t *p = g.b.p + (M::kSegments == 3 && cb.seg == 0 ? g.b.part : 0) + n0 * g.b.pitch;
+    const uint16_t *p = g.b.p + (M::kSegments == 3 && cb.seg == 0 ? g.b.part : 0) + n0 * g.b.row + cb.step * g.b.step;
     const __amdgpu_buffer_rsrc_t r =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, cb.left > 0 ? bytes_b : 0, 0x00020000);
     uint16_t *to = lds_b + cb.slot * Tile::kStageB + (wave + j * Tile::kWaves) * 8 * kStepK;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_b[j], cb.step * (kStepK * 2), 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_b[j], 0, 0, 0);
   };
   // One period of loads, from one meeting of the waves to the next: B's next step, then A's next (the one after, where A
   // has three stages).  They are issued a few at a time between the matrix instructions of the period's first kQuarters
