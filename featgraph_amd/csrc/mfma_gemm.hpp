@@ -178,49 +178,57 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
     off_b[j] = row * pitch_b + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
   }
-  // bytes in range: the rows that are there, of each the line of this step
-  const uint32_t bytes_b = static_cast<uint32_t>(min<int64_t>(Tile::BN, g.b.rows - n0) - 1) * pitch_b + kStepK * 2;
-
   const int total = g.steps * M::kSegments;
   const int first = static_cast<int>(static_cast<int64_t>(total) * at.split / g.splits);
   const int last = static_cast<int>(static_cast<int64_t>(total) * (at.split + 1) / g.splits);
   const int per_tile = last - first, n = per_tile * tiles;
-  // Loads of one step of an operand: its parts (segment 0 is hi * lo, 1 is lo * hi, 2 or the only one hi * hi), its k, its
-  // tile and its stage.  Past the last step nothing is fetched (no bytes are in range), so that the loop has no branches
-  // around its loads and always the same number of them under way.
+  // Where the next loads of an operand come from and go to: its part (segment 0 is hi * lo, 1 is lo * hi, 2 or the only one
+  // hi * hi), step and tile, with the address and the bytes in range (the rows that are there, of each the line of this
+  // step) kept up to date.  Past the last step nothing is in range, so that the loop has no branches around its loads and
+  // always the same number of them under way.
   struct Cursor {
-    int seg, step, slot, left, tile_left;
-    int64_t m;
+    const uint16_t *p;
+    int bytes, seg, slot, left, tile_left, until;  // until: steps before p has to be taken anew
   };
   const int first_seg = first / g.steps, first_step = first - first_seg * g.steps;
-  Cursor ca{first_seg, first_step, 0, n, per_tile, m0}, cb = ca;
-  auto advance = [&](Cursor &c, int stages) {
-    --c.left;
-    if (++c.step == g.steps) {
-      c.step = 0;
-      ++c.seg;
-    }
-    if (--c.tile_left == 0) {
-      c.tile_left = per_tile;
-      c.seg = first_seg;
-      c.step = first_step;
-      c.m += Tile::BM;
-    }
-    if (++c.slot == stages) c.slot = 0;
+  int64_t m_a = m0;  // first row of the tile that cursor a is in
+  auto begin = [&](Cursor &c, const GemmOperand &o, int64_t row, int rows, int step, int hi_segment) {
+    c.p = o.p + (M::kSegments == 3 && c.seg == hi_segment ? o.part : 0) + row * o.row + step * o.step;
+    c.bytes = static_cast<int>(min<int64_t>(rows, o.rows - row) - 1) * static_cast<int>(o.row * 2) + kStepK * 2;
+    c.until = min(g.steps - step, c.tile_left);
   };
+  auto advance = [&](Cursor &c, const GemmOperand &o, int64_t &row, int rows, int stride, int hi_segment, int stages) {
+    if (++c.slot == stages) c.slot = 0;
+    c.p += o.step;
+    --c.tile_left;
+    if (--c.left <= 0) {
+      c.bytes = 0;
+    } else if (--c.until == 0) {
+      int step = 0;
+      ++c.seg;
+      if (c.tile_left == 0) {
+        c.tile_left = per_tile;
+        c.seg = first_seg;
+        step = first_step;
+        row += stride;
+      }
+      begin(c, o, row, rows, step, hi_segment);
+    }
+  };
+  Cursor ca{nullptr, 0, first_seg, 0, n, per_tile, 0}, cb = ca;
+  int64_t m_b = n0;
+  begin(ca, g.a, m_a, Tile::BM, first_step, 1);
+  begin(cb, g.b, m_b, Tile::BN, first_step, 0);
+  auto advance_a = [&]() { advance(ca, g.a, m_a, Tile::BM, Tile::BM, 1, Tile::kStagesA); };
+  auto advance_b = [&]() { advance(cb, g.b, m_b, Tile::BN, 0, 0, 2); };
   uint16_t *const lds_b = lds + Tile::kStagesA * Tile::kStageA;
   auto load_a = [&](int j) {
-    const uint16_t *p = g.a.p + (M::kSegments == 3 && ca.seg == 1 ? g.a.part : 0) + ca.m * g.a.row + ca.step * g.a.step;
-    const uint32_t bytes_a = static_cast<uint32_t>(min<int64_t>(Tile::BM, g.a.rows - ca.m) - 1) * pitch_a + kStepK * 2;
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, ca.left > 0 ? bytes_a : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(ca.p), 0, ca.bytes, 0x00020000);
     uint16_t *to = lds + ca.slot * Tile::kStageA + (wave + j * Tile::kWaves) * 8 * kStepK;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_a[j], 0, 0, 0);
   };
   auto load_b = [&](int j) {
-    const uint16_t *p = g.b.p + (M::kSegments == 3 && cb.seg == 0 ? g.b.part : 0) + n0 * g.b.row + cb.step * g.b.step;
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(p), 0, cb.left > 0 ? bytes_b : 0, 0x00020000);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(cb.p), 0, cb.bytes, 0x00020000);
     uint16_t *to = lds_b + cb.slot * Tile::kStageB + (wave + j * Tile::kWaves) * 8 * kStepK;
     __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)to, 16, off_b[j], 0, 0, 0);
   };
@@ -232,8 +240,8 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
   auto load_one = [&](int l) {
     if (l < Tile::kLoadsB) load_b(l);
     else if (l < kLoads) load_a(l - Tile::kLoadsB);
-    if (l == Tile::kLoadsB - 1) advance(cb, 2);
-    if (l == kLoads - 1) advance(ca, Tile::kStagesA);
+    if (l == Tile::kLoadsB - 1) advance_b();
+    if (l == kLoads - 1) advance_a();
   };
 
   // fragments: lane l holds row l % 32, eight k from 16 * quarter + 8 * (l / 32) on
@@ -284,14 +292,14 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
   Fragments f0, f1;
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsA; ++j) load_a(j);
-  advance(ca, Tile::kStagesA);
+  advance_a();
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsB; ++j) load_b(j);
-  advance(cb, 2);
+  advance_b();
   if constexpr (kDeep) {
 #pragma unroll
     for (int j = 0; j < Tile::kLoadsA; ++j) load_a(j);
-    advance(ca, Tile::kStagesA);
+    advance_a();
   }
 #pragma unroll
   for (int l = 0; l < kPerQuarter; ++l) load_one(l);
