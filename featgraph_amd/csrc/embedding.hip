@@ -10,17 +10,18 @@
 // id (stably, so equal ids keep their order), the sorted list is cut into chunks, a group of lanes walks each chunk
 // and adds the rows of each run.  A run inside one chunk is written out at once; of a run that crosses a chunk's
 // border each chunk leaves a partial row (at most two per chunk: its first and its last run), and the partial rows,
-// again a sorted list, are added the same way.  The order of every sum depends on the ids and the sizes alone.
+// again a sorted list, are added the same way until few are left.  The order of every sum depends on the ids and the sizes alone.
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 #include "element.hpp"
 
 namespace fg {
 namespace {
 
-constexpr int kRankSortMost = 8192;   // ids that the one-launch sort takes (32 KB of LDS)
-constexpr int kRadixItems = 2048;     // ids per workgroup of the radix sort
+constexpr int kRankSortMost = 16384;  // ids that the one-launch sort takes (64 KB of LDS)
+constexpr int kRankThreads = 1024;
 constexpr int kRadixBits = 11;        // most bits per pass
 constexpr int32_t kSkip = INT32_MIN;  // flag on a partial row's key: nothing there to add
 
@@ -34,6 +35,7 @@ template <typename Id>
 __device__ __forceinline__ int32_t key_of(Id id, int32_t V) {
   return id >= 0 && id < static_cast<Id>(V) ? static_cast<int32_t>(id) : V;
 }
+__device__ __forceinline__ int32_t key_of(int2 entry, int32_t) { return entry.x; }  // of a list sorted before
 
 // ------------------------------------------------------------------------------------------------ lookup
 // A group of lpr lanes copies kRows rows at a time, each lane VEC elements of each: all ids first, then all rows,
@@ -49,7 +51,7 @@ __global__ __launch_bounds__(kBlockThreads) void lookup_kernel(const T *table, c
   if (first >= n) return;
   int32_t key[kRows];
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) key[r] = first + r < n ? key_of<Id>(ids[first + r], V) : V;
+  for (int r = 0; r < kRows; ++r) key[r] = first + r < n ? key_of(ids[first + r], V) : V;
   for (int32_t c = (blockIdx.y * lpr + sub) * VEC; c < D; c += gridDim.y * lpr * VEC) {
     P x[kRows];
 #pragma unroll
@@ -68,21 +70,22 @@ __global__ __launch_bounds__(kBlockThreads) void lookup_kernel(const T *table, c
 
 // ------------------------------------------------------------------------------------------------ sort
 // Up to kRankSortMost ids: the place of id i is the number of ids below it plus the number of equal ids before it,
-// counted directly.  A workgroup holds all ids in LDS and places 64 of them; each of its four waves counts over a
-// quarter of the list, four ids per LDS read.  N * N / 64 wave steps, but one launch.
+// counted directly.  A workgroup holds all ids in LDS and places 64 of them; each of its 16 waves counts over a
+// sixteenth of the list, four ids per LDS read.  N * N / 64 wave steps, but one launch (5 us for 333 ids, 20 for 16384,
+// where the six launches of the radix sort take 30).
 template <typename Id>
-__global__ __launch_bounds__(kBlockThreads) void rank_sort_kernel(const Id *ids, int32_t n, int32_t V, int32_t *keys,
-                                                                  int32_t *pos) {
+__global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(const Id *ids, int32_t n, int32_t V, int2 *sorted) {
+  constexpr int kWaves = kRankThreads / kWaveSize;
   __shared__ int4 all[kRankSortMost / 4];
-  __shared__ int32_t count[kWavesPerBlock][kWaveSize];
+  __shared__ int32_t count[kWaves][kWaveSize];
   int32_t *flat = reinterpret_cast<int32_t *>(all);
-  const int padded = (n + 15) & ~15;
-  for (int j = threadIdx.x; j < padded; j += kBlockThreads) flat[j] = j < n ? key_of<Id>(ids[j], V) : INT32_MAX;
+  const int padded = (n + 4 * kWaves - 1) / (4 * kWaves) * (4 * kWaves);
+  for (int j = threadIdx.x; j < padded; j += kRankThreads) flat[j] = j < n ? key_of(ids[j], V) : INT32_MAX;
   __syncthreads();
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int base = blockIdx.x * kWaveSize, i = base + lane;
   const int32_t mine = i < n ? flat[i] : -1;
-  const int quads = padded / 4, share = quads / kWavesPerBlock;
+  const int quads = padded / 4, share = quads / kWaves;
   int32_t below = 0;
   int q = wave * share;
   const int end = q + share;
@@ -103,26 +106,28 @@ __global__ __launch_bounds__(kBlockThreads) void rank_sort_kernel(const Id *ids,
   count[wave][lane] = below;
   __syncthreads();
   if (wave == 0 && i < n) {
-    const int place = count[0][lane] + count[1][lane] + count[2][lane] + count[3][lane];
-    keys[place] = mine;
-    pos[place] = i;
+    int place = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) place += count[w][lane];
+    sorted[place] = int2{mine, i};
   }
 }
 
+// The sorted list holds {key, position} pairs, which a scatter writes in one piece.
 // More ids: least-significant-digit radix sort, digits of up to kRadixBits bits (two passes up to 4M rows), three
 // launches per pass: counts per workgroup and digit, a scan of each digit's counts over the workgroups, the scatter.
-template <typename Id>
+template <typename Id, int kItems>
 __global__ __launch_bounds__(kBlockThreads) void radix_count_kernel(const Id *keys, int32_t n, int32_t V, int shift,
                                                                     int bits, int32_t *counts) {
   __shared__ int32_t hist[1 << kRadixBits];
   const int digits = 1 << bits;
   for (int d = threadIdx.x; d < digits; d += kBlockThreads) hist[d] = 0;
   __syncthreads();
-  const int32_t lo = blockIdx.x * kRadixItems;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kItems;
 #pragma unroll
-  for (int r = 0; r < kRadixItems / kBlockThreads; ++r) {
-    const int64_t i = static_cast<int64_t>(lo) + r * kBlockThreads + threadIdx.x;
-    if (i < n) atomicAdd(&hist[(key_of<Id>(keys[i], V) >> shift) & (digits - 1)], 1);
+  for (int r = 0; r < kItems / kBlockThreads; ++r) {
+    const int64_t i = lo + r * kBlockThreads + threadIdx.x;
+    if (i < n) atomicAdd(&hist[(key_of(keys[i], V) >> shift) & (digits - 1)], 1);
   }
   __syncthreads();
   for (int d = threadIdx.x; d < digits; d += kBlockThreads)
@@ -151,18 +156,31 @@ __global__ __launch_bounds__(kBlockThreads) void radix_scan_kernel(int32_t *coun
   if (lane == 0) totals[d] = before;
 }
 
-// A wave ranks its consecutive kRadixItems / 4 keys, 64 at a time: lanes of equal digit find each other by one ballot
+// A wave ranks its consecutive kItems / 4 keys, 64 at a time: lanes of equal digit find each other by one ballot
 // per bit, the first of them takes their places from the wave's counter of that digit.
-template <typename Id, bool kFirst>
-__global__ __launch_bounds__(kBlockThreads) void radix_scatter_kernel(const Id *keys, const int32_t *pos, int32_t n,
-                                                                      int32_t V, int shift, int bits,
-                                                                      const int32_t *counts, const int32_t *totals,
-                                                                      int32_t *keys_out, int32_t *pos_out) {
-  constexpr int kMost = 1 << kRadixBits, kRounds = kRadixItems / kBlockThreads;
+template <typename Id, bool kFirst, int kItems>
+__global__ __launch_bounds__(kBlockThreads) void radix_scatter_kernel(const Id *keys, int32_t n, int32_t V, int shift,
+                                                                      int bits, const int32_t *counts,
+                                                                      const int32_t *totals, int2 *sorted) {
+  constexpr int kMost = 1 << kRadixBits, kRounds = kItems / kBlockThreads;
   __shared__ int32_t taken[kWavesPerBlock][kMost];  // per wave and digit: keys ranked so far
   __shared__ int32_t base[kMost];                   // first place of each digit for this workgroup
   __shared__ int32_t sums[kBlockThreads];
   const int digits = 1 << bits, lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kItems + wave * (kItems / kWavesPerBlock);
+  int32_t key[kRounds], from[kRounds], rank[kRounds];
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    const int64_t i = lo + r * kWaveSize + lane;
+    key[r] = 0;
+    from[r] = -1;
+    if (i < n) {
+      const Id x = keys[i];
+      key[r] = key_of(x, V);
+      if constexpr (kFirst) from[r] = static_cast<int32_t>(i);
+      else from[r] = x.y;
+    }
+  }
   for (int d = threadIdx.x; d < digits; d += kBlockThreads) {
     base[d] = totals[d];
 #pragma unroll
@@ -189,14 +207,6 @@ __global__ __launch_bounds__(kBlockThreads) void radix_scatter_kernel(const Id *
       before += x;
     }
   }
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kRadixItems + wave * (kRadixItems / kWavesPerBlock);
-  int32_t key[kRounds], from[kRounds], rank[kRounds];
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    const int64_t i = lo + r * kWaveSize + lane;
-    key[r] = i < n ? key_of<Id>(keys[i], V) : 0;
-    from[r] = i < n ? (kFirst ? static_cast<int32_t>(i) : pos[i]) : -1;
-  }
 #pragma unroll
   for (int r = 0; r < kRounds; ++r) {
     const int d = (key[r] >> shift) & (digits - 1);
@@ -217,8 +227,7 @@ __global__ __launch_bounds__(kBlockThreads) void radix_scatter_kernel(const Id *
     const int d = (key[r] >> shift) & (digits - 1);
     int32_t place = base[d] + rank[r];
     for (int w = 0; w < wave; ++w) place += taken[w][d];
-    keys_out[place] = key[r];
-    pos_out[place] = from[r];
+    sorted[place] = int2{key[r], from[r]};
   }
 }
 
@@ -239,30 +248,62 @@ __device__ __forceinline__ void write_row(T *grad, int64_t at, const float *acc,
 }
 
 struct RunArgs {
-  const int32_t *keys;  // [n] ascending (partial rows: with kSkip set where there is nothing to add)
-  const int32_t *pos;   // [n] row of each entry (null: the entry's own place)
+  const int2 *sorted;   // [n] first level: {key, row}, keys ascending
+  const int32_t *keys;  // [n] later levels: keys of the rows, ascending, with kSkip set where there is nothing to add
   int64_t n;
   int32_t chunk;        // entries per group
   int32_t V, D;
   int lpr, accumulate;
+  int fill_blocks;      // workgroups ahead of the others that write zeros into the absent rows
   float scale;
   float *part;          // [2 * chunks, D] partial rows, slots 2c and 2c + 1 for the first and last run of chunk c
   int32_t *part_keys;   // [2 * chunks]
 };
 
-// S: element type of the rows that are added (the gradient's own, or float for partial rows).
-template <typename S, typename T, int VEC>
+// Zeros in the rows that no id names.  A wave looks 64 rows up in the sorted ids (one binary search per lane), then
+// writes those of them that are absent.
+template <typename T, int VEC>
+__device__ __forceinline__ void zero_absent(const int2 *sorted, int32_t n, int32_t V, int32_t D, int lpr, T *grad) {
+  using P = Pack<T, VEC>;
+  const int lane = threadIdx.x & (kWaveSize - 1), sub = lane & (lpr - 1);
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWaveSize) * kWaveSize;
+  if (r0 >= V) return;
+  int32_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int32_t m = lo + (hi - lo) / 2;
+    if (sorted[m].x < r0 + lane) lo = m + 1; else hi = m;
+  }
+  const uint64_t present = __ballot(lo < n && sorted[lo].x == r0 + lane);
+  P z;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) z.v[k] = narrow<T>(0.0f);
+  for (int r = lane / lpr; r < kWaveSize && r0 + r < V; r += kWaveSize / lpr) {
+    if ((present >> r) & 1) continue;
+    for (int32_t c = sub * VEC; c < D; c += lpr * VEC) *reinterpret_cast<P *>(grad + (r0 + r) * D + c) = z;
+  }
+}
+
+// S: element type of the rows that are added (the gradient's own on the first level, then float).
+template <typename S, typename T, int VEC, bool kFirst>
 __global__ __launch_bounds__(kBlockThreads) void run_sums_kernel(RunArgs a, const S *rows, T *grad) {
-  constexpr int kAhead = 4;
+  if (static_cast<int>(blockIdx.x) < a.fill_blocks) {
+    if (blockIdx.y == 0) zero_absent<T, VEC>(a.sorted, static_cast<int32_t>(a.n), a.V, a.D, a.lpr, grad);
+    return;
+  }
+  constexpr int kAhead = 8;  // rows under way per lane
   using P = Pack<S, VEC>;
   const int sub = threadIdx.x & (a.lpr - 1);
-  const int64_t c = (static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x) / a.lpr;
+  const int64_t c = ((static_cast<int64_t>(blockIdx.x) - a.fill_blocks) * kBlockThreads + threadIdx.x) / a.lpr;
   const int64_t lo = c * a.chunk, hi = min(lo + a.chunk, a.n);
   if (lo >= a.n) return;
   const int32_t col = (blockIdx.y * a.lpr + sub) * VEC;
   const bool mine = col < a.D, keeper = blockIdx.y == 0 && sub == 0;
-  const int32_t prev = lo > 0 ? a.keys[lo - 1] & ~kSkip : -1, next = hi < a.n ? a.keys[hi] & ~kSkip : -1;
-  int32_t cur = a.keys[lo] & ~kSkip;
+  auto entry = [&](int64_t e) {
+    if constexpr (kFirst) return a.sorted[e];
+    else return int2{a.keys[e], 0};
+  };
+  const int32_t prev = lo > 0 ? entry(lo - 1).x & ~kSkip : -1, next = hi < a.n ? entry(hi).x & ~kSkip : -1;
+  int32_t cur = entry(lo).x & ~kSkip;
   const int32_t first_key = cur;
   bool first = true, any = false, head = false, tail = false;  // head / tail: the two slots hold something
   float acc[VEC] = {};
@@ -282,14 +323,18 @@ __global__ __launch_bounds__(kBlockThreads) void run_sums_kernel(RunArgs a, cons
     }
   };
   for (int64_t e = lo; e < hi; e += kAhead) {
-    int32_t key[kAhead];
+    int32_t key[kAhead], row[kAhead];
     P x[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) key[u] = e + u < hi ? a.keys[e + u] : a.V;
+    for (int u = 0; u < kAhead; ++u) {
+      const int2 y = e + u < hi ? entry(e + u) : int2{a.V, 0};
+      key[u] = y.x;
+      row[u] = y.y;
+    }
 #pragma unroll
     for (int u = 0; u < kAhead; ++u)
       if (key[u] >= 0 && key[u] < a.V && mine) {
-        const int64_t r = a.pos ? a.pos[e + u] : e + u;
+        const int64_t r = kFirst ? row[u] : e + u;
         x[u] = *reinterpret_cast<const P *>(rows + r * a.D + col);
       }
 #pragma unroll
@@ -329,79 +374,70 @@ __global__ __launch_bounds__(kBlockThreads) void run_join_kernel(RunArgs a, cons
   if (k >= a.V || (e0 > 0 && (a.keys[e0 - 1] & ~kSkip) == k)) return;
   const int32_t col = (blockIdx.y * a.lpr + sub) * VEC;
   if (col >= a.D) return;
+  constexpr int kAhead = 8;
   float acc[VEC] = {};
-  bool any = false;
-  for (int64_t e = e0; e < a.n; ++e) {
-    const int32_t key = a.keys[e];
-    if ((key & ~kSkip) != k) break;
-    if (key < 0) continue;
-    any = true;
+  bool any = false, more = true;
+  for (int64_t e = e0; more && e < a.n; e += kAhead) {
+    int32_t key[kAhead];
+    Pack<float, VEC> x[kAhead];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] += rows[e * a.D + col + j];
+    for (int u = 0; u < kAhead; ++u) {
+      key[u] = e + u < a.n ? a.keys[e + u] : -1;
+      if (e + u < a.n) x[u] = *reinterpret_cast<const Pack<float, VEC> *>(rows + (e + u) * a.D + col);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      more = more && e + u < a.n && (key[u] & ~kSkip) == k;
+      if (!more || key[u] < 0) continue;
+      any = true;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[j] += x[u].v[j];
+    }
   }
   if (any) write_row<T, VEC>(grad, static_cast<int64_t>(k) * a.D + col, acc, a.scale, a.accumulate);
-}
-
-// Zeros in the rows that no id names.  A wave looks 64 rows up in the sorted ids (one binary search per lane), then
-// writes those of them that are absent.
-template <typename T, int VEC>
-__global__ __launch_bounds__(kBlockThreads) void zero_absent_kernel(const int32_t *keys, int32_t n, int32_t V,
-                                                                    int32_t D, int lpr, T *grad) {
-  using P = Pack<T, VEC>;
-  const int lane = threadIdx.x & (kWaveSize - 1), sub = lane & (lpr - 1);
-  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWaveSize) * kWaveSize;
-  if (r0 >= V) return;
-  int32_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int32_t m = lo + (hi - lo) / 2;
-    if (keys[m] < r0 + lane) lo = m + 1; else hi = m;
-  }
-  const uint64_t present = __ballot(lo < n && keys[lo] == r0 + lane);
-  P z;
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) z.v[k] = narrow<T>(0.0f);
-  for (int r = lane / lpr; r < kWaveSize && r0 + r < V; r += kWaveSize / lpr) {
-    if ((present >> r) & 1) continue;
-    for (int32_t c = sub * VEC; c < D; c += lpr * VEC) *reinterpret_cast<P *>(grad + (r0 + r) * D + c) = z;
-  }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
 int64_t align256(int64_t b) { return (b + 255) & ~int64_t{255}; }
 
+// Ids per workgroup of the radix sort: few for a short list, which would not fill the device, more for a long one, whose
+// counts per workgroup and digit are traffic (164,864 ids: 36 us with 1024, 44 with 2048; 1,000,003: 150 and 120).
+int radix_items(int64_t n) { return n <= 524288 ? 1024 : 4096; }
+
 // Entries per group on the first level: short chunks where the list is short (more groups in flight), longer ones
 // where it is long (fewer partial rows).
-int32_t chunk_of(int64_t n) { return n <= 65536 ? 16 : n <= 524288 ? 32 : 64; }
-constexpr int32_t kSecondChunk = 64;
-constexpr int64_t kJoinMost = 512;  // partial rows from which a second level runs before the join
+int32_t chunk_of(int64_t n) { return n <= 8192 ? 4 : n <= 65536 ? 8 : n <= 524288 ? 16 : 64; }
+constexpr int32_t kNextChunk = 8;    // ... on the levels after it
+constexpr int64_t kJoinMost = 2048;  // partial rows that one group may have to join at the end (all ids equal)
+constexpr int kMostLevels = 14;      // each leaves a quarter of the partial rows
 
 struct GradLayout {
-  int64_t keys[2], pos[2], counts, totals, part1, part1_keys, part2, part2_keys, bytes;
-  int64_t chunks1, chunks2;
+  int64_t sorted[2], counts, totals, bytes;
+  int levels;
+  int64_t chunks[kMostLevels], part[kMostLevels], part_keys[kMostLevels];
 };
 
 GradLayout grad_layout(int64_t n, int64_t D) {
-  GradLayout g;
+  GradLayout g{};
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
     at += align256(bytes);
     return here;
   };
-  g.chunks1 = (n + chunk_of(n) - 1) / chunk_of(n);
-  const int64_t e2 = 2 * g.chunks1;
-  g.chunks2 = e2 > kJoinMost ? (e2 + kSecondChunk - 1) / kSecondChunk : 0;
-  const int64_t blocks = (n + kRadixItems - 1) / kRadixItems;
-  for (int k = 0; k < 2; ++k) {
-    g.keys[k] = take(n * 4);
-    g.pos[k] = take(n * 4);
-  }
+  const int64_t blocks = (n + radix_items(n) - 1) / radix_items(n);
+  for (int k = 0; k < 2; ++k) g.sorted[k] = take(n * 8);
   g.counts = take(n > kRankSortMost ? blocks * (int64_t{4} << kRadixBits) : 0);
   g.totals = take(int64_t{4} << kRadixBits);
-  g.part1 = take(2 * g.chunks1 * D * 4);
-  g.part1_keys = take(2 * g.chunks1 * 4);
-  g.part2 = take(2 * g.chunks2 * D * 4);
-  g.part2_keys = take(2 * g.chunks2 * 4);
+  int64_t entries = n;
+  while (g.levels == 0 || entries > kJoinMost) {
+    const int32_t chunk = g.levels ? kNextChunk : chunk_of(n);
+    g.chunks[g.levels] = (entries + chunk - 1) / chunk;
+    entries = 2 * g.chunks[g.levels];
+    g.part[g.levels] = take(entries * D * 4);
+    g.part_keys[g.levels] = take(entries * 4);
+    ++g.levels;
+  }
   g.bytes = at;
   return g;
 }
@@ -412,86 +448,77 @@ unsigned blocks_for(int64_t groups, int lpr) {
 }
 
 template <typename Id>
-int sort_ids(const Id *ids, int32_t n, int32_t V, char *ws, const GradLayout &g, const int32_t **keys,
-             const int32_t **pos, hipStream_t stream) {
-  auto *k0 = reinterpret_cast<int32_t *>(ws + g.keys[0]), *k1 = reinterpret_cast<int32_t *>(ws + g.keys[1]);
-  auto *p0 = reinterpret_cast<int32_t *>(ws + g.pos[0]), *p1 = reinterpret_cast<int32_t *>(ws + g.pos[1]);
+int sort_ids(const Id *ids, int32_t n, int32_t V, char *ws, const GradLayout &g, const int2 **sorted, hipStream_t stream) {
+  auto *s0 = reinterpret_cast<int2 *>(ws + g.sorted[0]), *s1 = reinterpret_cast<int2 *>(ws + g.sorted[1]);
   if (n <= kRankSortMost) {
-    rank_sort_kernel<Id><<<dim3((n + kWaveSize - 1) / kWaveSize), dim3(kBlockThreads), 0, stream>>>(ids, n, V, k0, p0);
+    rank_sort_kernel<Id><<<dim3((n + kWaveSize - 1) / kWaveSize), dim3(kRankThreads), 0, stream>>>(ids, n, V, s0);
     FG_HIP_TRY(hipGetLastError());
-    *keys = k0;
-    *pos = p0;
+    *sorted = s0;
     return FG_OK;
   }
   int total_bits = 1;
   while (total_bits < 31 && (V >> total_bits) != 0) ++total_bits;  // keys 0 .. V
   const int passes = (total_bits + kRadixBits - 1) / kRadixBits, bits = (total_bits + passes - 1) / passes;
-  const int32_t blocks = static_cast<int32_t>((static_cast<int64_t>(n) + kRadixItems - 1) / kRadixItems);
+  const int32_t blocks = static_cast<int32_t>((static_cast<int64_t>(n) + radix_items(n) - 1) / radix_items(n));
   auto *counts = reinterpret_cast<int32_t *>(ws + g.counts), *totals = reinterpret_cast<int32_t *>(ws + g.totals);
-  for (int p = 0; p < passes; ++p) {
-    const int shift = p * bits;
-    if (p == 0)
-      radix_count_kernel<Id><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(ids, n, V, shift, bits, counts);
-    else
-      radix_count_kernel<int32_t><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(k0, n, V, shift, bits, counts);
-    radix_scan_kernel<<<dim3(((1 << bits) + kWavesPerBlock - 1) / kWavesPerBlock), dim3(kBlockThreads), 0, stream>>>(
-        counts, blocks, 1 << bits, totals);
-    if (p == 0)
-      radix_scatter_kernel<Id, true><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(ids, nullptr, n, V, shift, bits,
-                                                                                       counts, totals, k1, p1);
-    else
-      radix_scatter_kernel<int32_t, false><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(
-          k0, p0, n, V, shift, bits, counts, totals, k1, p1);
-    std::swap(k0, k1);
-    std::swap(p0, p1);
-  }
+  auto sort = [&](auto items) {
+    constexpr int kItems = decltype(items)::value;
+    for (int p = 0; p < passes; ++p) {
+      const int shift = p * bits;
+      if (p == 0)
+        radix_count_kernel<Id, kItems><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(ids, n, V, shift, bits, counts);
+      else
+        radix_count_kernel<int2, kItems><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(s0, n, V, shift, bits, counts);
+      radix_scan_kernel<<<dim3(((1 << bits) + kWavesPerBlock - 1) / kWavesPerBlock), dim3(kBlockThreads), 0, stream>>>(
+          counts, blocks, 1 << bits, totals);
+      if (p == 0)
+        radix_scatter_kernel<Id, true, kItems><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(
+            ids, n, V, shift, bits, counts, totals, s1);
+      else
+        radix_scatter_kernel<int2, false, kItems><<<dim3(blocks), dim3(kBlockThreads), 0, stream>>>(
+            s0, n, V, shift, bits, counts, totals, s1);
+      std::swap(s0, s1);
+    }
+  };
+  if (radix_items(n) == 1024) sort(std::integral_constant<int, 1024>{});
+  else sort(std::integral_constant<int, 4096>{});
   FG_HIP_TRY(hipGetLastError());
-  *keys = k0;
-  *pos = p0;
+  *sorted = s0;
   return FG_OK;
 }
 
 template <typename T, int VEC>
-int grad_rows(const int32_t *keys, const int32_t *pos, int64_t n, int64_t V, int64_t D, const T *dout, T *grad,
+int grad_rows(const int2 *sorted, int64_t n, int64_t V, int64_t D, const T *dout, T *grad,
               float scale, int accumulate, char *ws, const GradLayout &g, hipStream_t stream) {
   const int lpr = lanes_per_row(D, VEC);
   const unsigned tiles = static_cast<unsigned>((D + lpr * VEC - 1) / (lpr * VEC));
-  if (!accumulate) {
-    const int64_t waves = (V + kWaveSize - 1) / kWaveSize;
-    zero_absent_kernel<T, VEC><<<dim3(static_cast<unsigned>((waves + kWavesPerBlock - 1) / kWavesPerBlock)),
-                                 dim3(kBlockThreads), 0, stream>>>(keys, static_cast<int32_t>(n),
-                                                                   static_cast<int32_t>(V), static_cast<int32_t>(D),
-                                                                   lpr, grad);
-  }
-  if (n == 0) {
-    FG_HIP_TRY(hipGetLastError());
-    return FG_OK;
-  }
   RunArgs a{};
-  a.keys = keys;
-  a.pos = pos;
+  a.sorted = sorted;
   a.n = n;
-  a.chunk = chunk_of(n);
   a.V = static_cast<int32_t>(V);
   a.D = static_cast<int32_t>(D);
   a.lpr = lpr;
   a.accumulate = accumulate;
   a.scale = scale;
-  a.part = reinterpret_cast<float *>(ws + g.part1);
-  a.part_keys = reinterpret_cast<int32_t *>(ws + g.part1_keys);
-  run_sums_kernel<T, T, VEC><<<dim3(blocks_for(g.chunks1, lpr), tiles), dim3(kBlockThreads), 0, stream>>>(a, dout, grad);
-  const float *rows = a.part;
-  a.keys = a.part_keys;
-  a.pos = nullptr;
-  a.n = 2 * g.chunks1;
-  if (g.chunks2) {
-    a.chunk = kSecondChunk;
-    a.part = reinterpret_cast<float *>(ws + g.part2);
-    a.part_keys = reinterpret_cast<int32_t *>(ws + g.part2_keys);
-    run_sums_kernel<float, T, VEC><<<dim3(blocks_for(g.chunks2, lpr), tiles), dim3(kBlockThreads), 0, stream>>>(a, rows, grad);
+  a.fill_blocks = accumulate ? 0 : static_cast<int>((V + kWaveSize * kWavesPerBlock - 1) / (kWaveSize * kWavesPerBlock));
+  const float *rows = nullptr;
+  for (int k = 0; k < g.levels; ++k) {
+    a.chunk = k ? kNextChunk : chunk_of(n);
+    a.part = reinterpret_cast<float *>(ws + g.part[k]);
+    a.part_keys = reinterpret_cast<int32_t *>(ws + g.part_keys[k]);
+    const dim3 grid(a.fill_blocks + blocks_for(g.chunks[k], lpr), tiles);
+    if (k == 0)
+      run_sums_kernel<T, T, VEC, true><<<grid, dim3(kBlockThreads), 0, stream>>>(a, dout, grad);
+    else
+      run_sums_kernel<float, T, VEC, false><<<grid, dim3(kBlockThreads), 0, stream>>>(a, rows, grad);
+    if (n == 0) {
+      FG_HIP_TRY(hipGetLastError());
+      return FG_OK;
+    }
     rows = a.part;
     a.keys = a.part_keys;
-    a.n = 2 * g.chunks2;
+    a.n = 2 * g.chunks[k];
+    a.fill_blocks = 0;
   }
   run_join_kernel<T, VEC><<<dim3(blocks_for(a.n, lpr), tiles), dim3(kBlockThreads), 0, stream>>>(a, rows, grad);
   FG_HIP_TRY(hipGetLastError());
@@ -499,17 +526,17 @@ int grad_rows(const int32_t *keys, const int32_t *pos, int64_t n, int64_t V, int
 }
 
 template <typename T>
-int grad_typed(const int32_t *keys, const int32_t *pos, int64_t n, int64_t V, int64_t D, const void *dout, void *grad,
+int grad_typed(const int2 *sorted, int64_t n, int64_t V, int64_t D, const void *dout, void *grad,
                float scale, int accumulate, char *ws, const GradLayout &g, hipStream_t stream) {
   const T *d = static_cast<const T *>(dout);
   T *o = static_cast<T *>(grad);
   switch (vector_elements(D, sizeof(T), {dout, grad})) {
     case 8:
-      if constexpr (sizeof(T) == 2) return grad_rows<T, 8>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
+      if constexpr (sizeof(T) == 2) return grad_rows<T, 8>(sorted, n, V, D, d, o, scale, accumulate, ws, g, stream);
       [[fallthrough]];
-    case 4: return grad_rows<T, 4>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
-    case 2: return grad_rows<T, 2>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
-    default: return grad_rows<T, 1>(keys, pos, n, V, D, d, o, scale, accumulate, ws, g, stream);
+    case 4: return grad_rows<T, 4>(sorted, n, V, D, d, o, scale, accumulate, ws, g, stream);
+    case 2: return grad_rows<T, 2>(sorted, n, V, D, d, o, scale, accumulate, ws, g, stream);
+    default: return grad_rows<T, 1>(sorted, n, V, D, d, o, scale, accumulate, ws, g, stream);
   }
 }
 
@@ -584,14 +611,14 @@ int fg_embedding_grad(int64_t n_rows, int64_t D, int64_t n_ids, const void *ids,
     return fg::fail(FG_EINVAL, "the workspace needs %lld bytes at a multiple of 256", (long long)g.bytes);
   hipStream_t s = static_cast<hipStream_t>(stream);
   char *ws = static_cast<char *>(workspace);
-  const int32_t *keys = reinterpret_cast<const int32_t *>(ws), *pos = keys;
+  const int2 *sorted = nullptr;
   if (n_ids > 0) {
     const int32_t n = static_cast<int32_t>(n_ids), V = static_cast<int32_t>(n_rows);
-    const int rc = itype == FG_I32 ? fg::sort_ids(static_cast<const int32_t *>(ids), n, V, ws, g, &keys, &pos, s)
-                                   : fg::sort_ids(static_cast<const int64_t *>(ids), n, V, ws, g, &keys, &pos, s);
+    const int rc = itype == FG_I32 ? fg::sort_ids(static_cast<const int32_t *>(ids), n, V, ws, g, &sorted, s)
+                                   : fg::sort_ids(static_cast<const int64_t *>(ids), n, V, ws, g, &sorted, s);
     if (rc) return rc;
   }
-#define FG_TYPED(T) fg::grad_typed<T>(keys, pos, n_ids, n_rows, D, dout, grad, scale, accumulate, ws, g, s)
+#define FG_TYPED(T) fg::grad_typed<T>(sorted, n_ids, n_rows, D, dout, grad, scale, accumulate, ws, g, s)
   if (dtype == FG_F32) return FG_TYPED(float);
   if (dtype == FG_BF16) return FG_TYPED(__bf16);
   return FG_TYPED(_Float16);
