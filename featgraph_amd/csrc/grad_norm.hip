@@ -3,11 +3,12 @@
 //   norm = sqrt(sum over tensors t, elements i of g_t[i]^2)      c = min(1, max_norm / (norm + eps))
 //   out_t[i] = c * g_t[i]
 //
-// All tensors of a call are one list of 16 KB pieces.  A workgroup takes a contiguous range of the list, so that it
+// All tensors of a call are one list of 8 KB pieces.  A workgroup takes a contiguous range of the list, so that it
 // looks its first tensor up once and then moves on; it adds squares in float64 (no overflow for any float32, and the
 // device's double rate is far above what memory delivers) and leaves one partial sum.  The scaling kernel's
 // workgroups each add the partial sums again, in the same order, which costs less than a launch between the two.
-// Small lists (the layers of a small model) run in one workgroup and one launch.  The tensors' addresses travel in
+// The scaling goes through each workgroup's range from its end: what the first pass read last is still in the last-level
+// cache.  Small lists (the layers of a small model) run in one workgroup and one launch.  The tensors' addresses travel in
 // the kernel arguments, so a call can be captured into a graph and needs no copy to the device.
 #include <algorithm>
 #include <initializer_list>
@@ -18,9 +19,9 @@ namespace fg {
 namespace {
 
 constexpr int kTensors = 96;          // per launch: 29 bytes each, within the 4 KB of kernel arguments
-constexpr int kPieceBytes = 16384;
+constexpr int kPieceBytes = 8192;
 constexpr int kMostBlocks = 2048;     // partial sums over all launches of a call
-constexpr int kSmallPieces = 16;      // pieces up to which one workgroup does everything
+constexpr int kSmallPieces = 16;      // pieces up to which one workgroup does everything, a wave each
 constexpr int kSmallThreads = 1024;
 
 struct TensorList {
@@ -47,6 +48,17 @@ __device__ __forceinline__ double block_sum(double x, double *lds) {
   return s;
 }
 
+template <typename T, int N>
+__device__ __forceinline__ double square_sum(const Pack<T, N> &p) {
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const double d = static_cast<double>(widen(p.v[k]));
+    s = __builtin_fma(d, d, s);
+  }
+  return s;
+}
+
 // Sum of squares of elements [lo, hi) of one tensor, this thread's share.
 template <typename T, int THREADS>
 __device__ __forceinline__ double squares(const void *in, int64_t lo, int64_t hi, bool aligned) {
@@ -57,14 +69,16 @@ __device__ __forceinline__ double squares(const void *in, int64_t lo, int64_t hi
   int64_t i = lo;
   if (aligned) {
     const int64_t whole = lo + (hi - lo) / kVec * kVec;
-    for (int64_t j = lo + threadIdx.x * kVec; j < whole; j += THREADS * kVec) {
-      const P p = *reinterpret_cast<const P *>(x + j);
+    constexpr int kUnroll = 4;
+    int64_t j = lo + threadIdx.x * kVec;
+    for (; j + THREADS * kVec * (kUnroll - 1) < whole; j += THREADS * kVec * kUnroll) {
+      P p[kUnroll];
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) {
-        const double d = static_cast<double>(widen(p.v[k]));
-        s = __builtin_fma(d, d, s);
-      }
+      for (int u = 0; u < kUnroll; ++u) p[u] = *reinterpret_cast<const P *>(x + j + THREADS * kVec * u);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) s += square_sum(p[u]);
     }
+    for (; j < whole; j += THREADS * kVec) s += square_sum(*reinterpret_cast<const P *>(x + j));
     i = whole;
   }
   for (int64_t j = i + threadIdx.x; j < hi; j += THREADS) {
@@ -74,28 +88,49 @@ __device__ __forceinline__ double squares(const void *in, int64_t lo, int64_t hi
   return s;
 }
 
+// A store that leaves the last-level cache to the gradients that are still to be read (3% of the two passes together).
+template <typename T, typename P>
+__device__ __forceinline__ void store_past(T *to, const P &p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4, p), reinterpret_cast<u32x4 *>(to));
+}
+
 template <typename T, int THREADS>
 __device__ __forceinline__ void scale_out(const void *in, void *out, int64_t lo, int64_t hi, bool aligned, float c) {
-  constexpr int kVec = 16 / sizeof(T);
+  constexpr int kVec = 16 / sizeof(T), kUnroll = 4;
   using P = Pack<T, kVec>;
   const T *x = static_cast<const T *>(in);
   T *y = static_cast<T *>(out);
-  int64_t i = lo;
   if (aligned) {
     const int64_t whole = lo + (hi - lo) / kVec * kVec;
-    for (int64_t j = lo + threadIdx.x * kVec; j < whole; j += THREADS * kVec) {
+    for (int64_t j = whole + threadIdx.x; j < hi; j += THREADS) y[j] = narrow<T>(widen(x[j]) * c);
+    int64_t end = whole;
+    for (; end - lo >= THREADS * kVec * kUnroll; end -= THREADS * kVec * kUnroll) {
+      P p[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        p[u] = *reinterpret_cast<const P *>(x + end - (THREADS * (u + 1) - threadIdx.x) * kVec);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) p[u].v[k] = narrow<T>(widen(p[u].v[k]) * c);
+        store_past(y + end - (THREADS * (u + 1) - threadIdx.x) * kVec, p[u]);
+      }
+    }
+    for (int64_t j = lo + threadIdx.x * kVec; j < end; j += THREADS * kVec) {
       P p = *reinterpret_cast<const P *>(x + j);
 #pragma unroll
       for (int k = 0; k < kVec; ++k) p.v[k] = narrow<T>(widen(p.v[k]) * c);
       *reinterpret_cast<P *>(y + j) = p;
     }
-    i = whole;
+    return;
   }
-  for (int64_t j = i + threadIdx.x; j < hi; j += THREADS) y[j] = narrow<T>(widen(x[j]) * c);
+  for (int64_t j = lo + threadIdx.x; j < hi; j += THREADS) y[j] = narrow<T>(widen(x[j]) * c);
 }
 
-// Calls f(tensor, first element, one past the last) for this workgroup's share of the list, tensor by tensor.
-template <typename F>
+// Calls f(tensor, first element, one past the last) for this workgroup's share of the list, tensor by tensor, from the
+// last tensor to the first with kBack.
+template <bool kBack, typename F>
 __device__ __forceinline__ void for_share(const TensorList &l, F &&f) {
   const int32_t total = l.first[l.count];
   const int32_t lo = static_cast<int32_t>(static_cast<int64_t>(total) * blockIdx.x / gridDim.x);
@@ -106,7 +141,10 @@ __device__ __forceinline__ void for_share(const TensorList &l, F &&f) {
     const int m = (a + b + 1) / 2;
     if (l.first[m] <= lo) a = m; else b = m - 1;
   }
-  for (int t = a; t < l.count && l.first[t] < hi; ++t) {
+  int z = a;  // one past the last tensor that starts below `hi`
+  while (z < l.count && l.first[z] < hi) ++z;
+  for (int k = a; k < z; ++k) {
+    const int t = kBack ? z - 1 - (k - a) : k;
     const int32_t p0 = max(lo, l.first[t]), p1 = min(hi, l.first[t + 1]);
     if (p0 >= p1) continue;
     const int64_t per = kPieceBytes / ((l.type[t] & 3) == FG_F32 ? 4 : 2);
@@ -117,7 +155,7 @@ __device__ __forceinline__ void for_share(const TensorList &l, F &&f) {
 template <int THREADS>
 __device__ __forceinline__ double share_squares(const TensorList &l) {
   double s = 0.0;
-  for_share(l, [&](int t, int64_t lo, int64_t hi) {
+  for_share<false>(l, [&](int t, int64_t lo, int64_t hi) {
     const int type = l.type[t] & 3;
     const bool aligned = l.type[t] < 4;
     if (type == FG_F32) s += squares<float, THREADS>(l.in[t], lo, hi, aligned);
@@ -129,7 +167,7 @@ __device__ __forceinline__ double share_squares(const TensorList &l) {
 
 template <int THREADS>
 __device__ __forceinline__ void share_scale(const TensorList &l, float c) {
-  for_share(l, [&](int t, int64_t lo, int64_t hi) {
+  for_share<true>(l, [&](int t, int64_t lo, int64_t hi) {
     const int type = l.type[t] & 3;
     const bool aligned = l.type[t] < 4;
     if (l.out[t] == l.in[t] && c == 1.0f) return;  // in place and nothing to clip
@@ -146,12 +184,64 @@ __device__ __forceinline__ float coefficient(double norm, float max_norm, float 
   return c < 1.0 || c != c ? static_cast<float>(c) : 1.0f;
 }
 
+// One wave per piece.  The piece stays in registers between the two passes (eight loads of 16 bytes per lane, all under way
+// at once); only a tensor off its alignment is read again.
 __global__ __launch_bounds__(kSmallThreads) void small_kernel(TensorList l, int clip, float max_norm, float eps,
                                                               float *norm_out) {
+  constexpr int kHeld = kPieceBytes / (kWaveSize * 16);
+  static_assert(kSmallPieces == kSmallThreads / kWaveSize, "a wave per piece");
   __shared__ double lds[kSmallThreads / kWaveSize];
-  const double norm = sqrt(block_sum<kSmallThreads>(share_squares<kSmallThreads>(l), lds));
+  const int lane = threadIdx.x & (kWaveSize - 1), piece = threadIdx.x / kWaveSize;
+  const bool busy = piece < l.first[l.count];
+  int t = 0;  // tensors that end at or before this piece: counted by the lanes together
+  for (int k = 0; k < l.count; k += kWaveSize)
+    t += __popcll(__ballot(k + lane < l.count && l.first[k + lane + 1] <= piece));
+  t = busy ? t : 0;
+  const int type = busy ? l.type[t] & 3 : 0, bytes = type == FG_F32 ? 4 : 2;
+  const bool aligned = busy && l.type[t] < 4;
+  const int64_t per = kPieceBytes / bytes, lo = busy ? (piece - l.first[t]) * per : 0;
+  const int count = busy ? static_cast<int>(min(per, l.n[t] - lo)) : 0;  // elements of this piece
+  const int vectors = aligned ? count * bytes / 16 : 0;                  // whole 16-byte vectors of it
+  const int loose = vectors * 16 / bytes;                                // first element behind them
+  const char *in = busy ? static_cast<const char *>(l.in[t]) + lo * bytes : nullptr;
+  char *out = busy && clip ? static_cast<char *>(l.out[t]) + lo * bytes : nullptr;
+  uint4 held[kHeld];
+#pragma unroll
+  for (int u = 0; u < kHeld; ++u)
+    held[u] = u * kWaveSize + lane < vectors ? reinterpret_cast<const uint4 *>(in)[u * kWaveSize + lane] : uint4{0, 0, 0, 0};
+  auto typed = [&](auto &&f) {  // f(a value of the tensor's type)
+    if (type == FG_F32) f(0.0f);
+    else if (type == FG_BF16) f(__bf16{});
+    else f(_Float16{});
+  };
+  double s = 0.0;
+  typed([&](auto kind) {
+    using T = decltype(kind);
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) s += square_sum(__builtin_bit_cast(Pack<T, 16 / sizeof(T)>, held[u]));
+    for (int j = loose + lane; j < count; j += kWaveSize) {
+      const double d = static_cast<double>(widen(reinterpret_cast<const T *>(in)[j]));
+      s = __builtin_fma(d, d, s);
+    }
+  });
+  const double norm = sqrt(block_sum<kSmallThreads>(s, lds));
   if (threadIdx.x == 0) *norm_out = static_cast<float>(norm);
-  if (clip) share_scale<kSmallThreads>(l, coefficient(norm, max_norm, eps));
+  if (!clip || !busy) return;
+  const float c = coefficient(norm, max_norm, eps);
+  if (in == out && c == 1.0f) return;  // in place and nothing to clip
+  typed([&](auto kind) {
+    using T = decltype(kind);
+    constexpr int kVec = 16 / sizeof(T);
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      auto p = __builtin_bit_cast(Pack<T, kVec>, held[u]);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) p.v[k] = narrow<T>(widen(p.v[k]) * c);
+      if (u * kWaveSize + lane < vectors) reinterpret_cast<Pack<T, kVec> *>(out)[u * kWaveSize + lane] = p;
+    }
+    for (int j = loose + lane; j < count; j += kWaveSize)
+      reinterpret_cast<T *>(out)[j] = narrow<T>(widen(reinterpret_cast<const T *>(in)[j]) * c);
+  });
 }
 
 __global__ __launch_bounds__(kBlockThreads) void squares_kernel(TensorList l, double *partial) {
