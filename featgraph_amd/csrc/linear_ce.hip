@@ -82,71 +82,104 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
   return u < 0x7f800000u ? u : 0u;
 }
 
+// One matrix to copy for the products; a launch takes two (h and a piece of w), either of which may have no blocks.
+struct CopyJob {
+  const void *x;            // [rows, D]
+  uint16_t *out;
+  int64_t rows;
+  int32_t D;
+  uint32_t blocks;          // of the launch
+  int32_t *exps;            // float32, row copy: exponents of the rows
+  uint32_t *peak;           // float32: the largest |x| * |factor[row]| of the rows that are kept; written by the row copy
+                            // (null: not wanted), read by the transposed copy
+  const int32_t *keep;      // rows whose keep[] is negative do not count in peak, and are zeros in the transposed copy
+  const float *factor;      // float32: per row, for peak and the transposed copy (null: 1)
+};
+struct CopyJobs {
+  CopyJob job[2];
+};
+// This block's job and its number in it.
+__device__ __forceinline__ const CopyJob &job_of(const CopyJobs &jobs, uint32_t *block) {
+  const bool second = blockIdx.x >= jobs.job[0].blocks;
+  *block = second ? blockIdx.x - jobs.job[0].blocks : blockIdx.x;
+  return jobs.job[second];
+}
+
 // bfloat16: [rows, D] -> panels
-__global__ __launch_bounds__(kBlockThreads) void pad_kernel(const uint16_t *x, uint16_t *out, int64_t rows, int32_t D) {
-  const int64_t total = rows * ((D + kStepK - 1) / kStepK * kStepK), stride = static_cast<int64_t>(gridDim.x) * kBlockThreads;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kBlockThreads + threadIdx.x; t < total; t += stride) {
-    const int64_t panel = t / (rows * kStepK), in_panel = t - panel * (rows * kStepK);
+__device__ __forceinline__ void pad_rows(const CopyJob &job, uint32_t block) {
+  const auto *x = static_cast<const uint16_t *>(job.x);
+  const int64_t per_panel = job.rows * kStepK;
+  const int64_t total = per_panel * ((job.D + kStepK - 1) / kStepK), stride = static_cast<int64_t>(job.blocks) * kBlockThreads;
+  for (int64_t t = static_cast<int64_t>(block) * kBlockThreads + threadIdx.x; t < total; t += stride) {
+    const int64_t panel = t / per_panel, in_panel = t - panel * per_panel;
     const int64_t c = panel * kStepK + in_panel % kStepK;
-    out[t] = c < D ? x[in_panel / kStepK * D + c] : 0;
+    job.out[t] = c < job.D ? x[in_panel / kStepK * job.D + c] : 0;
   }
 }
 
-// float32: [rows, D] -> two parts as panels, each row by its own exponent (exps).  One wave per row.
-// peak (or null): largest |x| * |factor[row]| over the rows whose keep[] is not negative, for the transposed copy.
-__global__ __launch_bounds__(kBlockThreads) void split_rows_kernel(const float *x, uint16_t *out, int64_t rows,
-                                                                   int32_t D, int32_t *exps, uint32_t *peak,
-                                                                   const int32_t *keep, const float *factor) {
+// float32: [rows, D] -> two parts as panels, each row by its own exponent.  One wave per row.
+__device__ __forceinline__ void split_rows(const CopyJob &job, uint32_t block) {
   __shared__ uint32_t peaks[kWavesPerBlock];
+  const auto *x = static_cast<const float *>(job.x);
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
-  const int32_t Dp = (D + kStepK - 1) / kStepK * kStepK;
-  const int64_t part = rows * Dp, stride = static_cast<int64_t>(gridDim.x) * kWavesPerBlock;
+  const int32_t D = job.D, padded = (D + kStepK - 1) / kStepK * kStepK;
+  const int64_t part = job.rows * padded, stride = static_cast<int64_t>(job.blocks) * kWavesPerBlock;
   uint32_t most = 0;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + wave; r < rows; r += stride) {
+  for (int64_t r = static_cast<int64_t>(block) * kWavesPerBlock + wave; r < job.rows; r += stride) {
     const float *row = x + r * D;
     uint32_t top = 0;
     for (int32_t c = lane; c < D; c += kWaveSize) top = max(top, finite_bits(row[c]));
 #pragma unroll
     for (int d = 1; d < kWaveSize; d <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, kWaveSize)));
     const int e = exponent_for(top);
-    if (lane == 0) exps[r] = e;
-    for (int32_t c = lane; c < Dp; c += kWaveSize) {
+    if (lane == 0) job.exps[r] = e;
+    for (int32_t c = lane; c < padded; c += kWaveSize) {
       const float y = c < D ? __builtin_ldexpf(row[c], e) : 0.0f;
-      const int64_t to = panel_at(rows, r, c);
-      out[to] = static_cast<uint16_t>(part_of<float>(y, 0));
-      out[part + to] = static_cast<uint16_t>(part_of<float>(y, 1));
+      const int64_t to = panel_at(job.rows, r, c);
+      job.out[to] = static_cast<uint16_t>(part_of<float>(y, 0));
+      job.out[part + to] = static_cast<uint16_t>(part_of<float>(y, 1));
     }
-    if (peak && (!keep || keep[r] >= 0))
-      most = max(most, finite_bits(__builtin_bit_cast(float, top) * (factor ? factor[r] : 1.0f)));
+    if (job.peak && (!job.keep || job.keep[r] >= 0))
+      most = max(most, finite_bits(__builtin_bit_cast(float, top) * (job.factor ? job.factor[r] : 1.0f)));
   }
-  if (!peak) return;
+  if (!job.peak) return;
   if (lane == 0) peaks[wave] = most;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kWavesPerBlock; ++w) most = max(most, peaks[w]);
-    atomicMax(peak + blockIdx.x % kPeakSlots * kPeakStride, most);  // a largest value does not depend on the order
+    atomicMax(job.peak + block % kPeakSlots * kPeakStride, most);  // a largest value does not depend on the order
   }
 }
 
-// [rows, D] -> parts of its transpose as panels of 64 rows' elements, zeros in place of rows whose keep[] is negative (whatever those
-// hold must not reach the sum over rows).  float32: times factor[row] (or 1) and brought into range by *peak.
+template <typename T>
+__global__ __launch_bounds__(kBlockThreads) void copy_rows_kernel(CopyJobs jobs) {
+  uint32_t block;
+  const CopyJob &job = job_of(jobs, &block);
+  if constexpr (sizeof(T) == 4) split_rows(job, block);
+  else pad_rows(job, block);
+}
+
+// [rows, D] -> parts of its transpose as panels of 64 rows' elements, zeros in place of rows whose keep[] is negative
+// (whatever those hold must not reach the sum over rows).  float32: times factor[row] and brought into range by *peak.
 // 64 x 64 elements per workgroup, 16 bytes per lane on both sides where D allows (kVec elements per load).
 template <typename T, int kVec>
-__global__ __launch_bounds__(kBlockThreads) void transpose_kernel(const T *x, const int32_t *keep, const float *factor,
-                                                                  const uint32_t *peak, uint16_t *out, int32_t rows,
-                                                                  int32_t D) {
+__global__ __launch_bounds__(kBlockThreads) void copy_transposed_kernel(CopyJobs jobs) {
   constexpr int kLanes = 64 / kVec;  // per row
   __shared__ float tile[64][65];
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
-  const int c0 = blockIdx.y * 64;
-  const int e = peak ? exponent_for(read_peak(peak)) : 0;
+  uint32_t block;
+  const CopyJob &job = job_of(jobs, &block);
+  const int64_t panels = (job.rows + kStepK - 1) / kStepK, panel = block % panels;
+  const int64_t r0 = panel * kStepK;
+  const int32_t D = job.D;
+  const int c0 = static_cast<int>(block / panels) * 64;
+  const int e = sizeof(T) == 4 ? exponent_for(read_peak(job.peak)) : 0;
   const int c = c0 + threadIdx.x % kLanes * kVec;
   for (int k = threadIdx.x / kLanes; k < 64; k += kBlockThreads / kLanes) {
     const int64_t r = r0 + k;
     Pack<T, kVec> v;
-    const bool there = r < rows && c < D && (!keep || keep[r] >= 0);
-    if (there) v = *reinterpret_cast<const Pack<T, kVec> *>(x + r * D + c);
-    const float f = sizeof(T) == 4 && there && factor ? factor[r] : 1.0f;
+    const bool there = r < job.rows && c < D && (!job.keep || job.keep[r] >= 0);
+    if (there) v = *reinterpret_cast<const Pack<T, kVec> *>(static_cast<const T *>(job.x) + r * D + c);
+    const float f = sizeof(T) == 4 && there && job.factor ? job.factor[r] : 1.0f;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       float y = there ? widen(v.v[j]) : 0.0f;
@@ -163,8 +196,7 @@ __global__ __launch_bounds__(kBlockThreads) void transpose_kernel(const T *x, co
       Pack<uint16_t, 8> y;
 #pragma unroll
       for (int k = 0; k < 8; ++k) y.v[k] = static_cast<uint16_t>(part_of<T>(tile[8 * g + k][col], p));
-      const int64_t panel = blockIdx.x + static_cast<int64_t>(p) * gridDim.x;  // a part has gridDim.x panels
-      *reinterpret_cast<Pack<uint16_t, 8> *>(out + (panel * D + c0 + col) * kStepK + 8 * g) = y;
+      *reinterpret_cast<Pack<uint16_t, 8> *>(job.out + ((panel + p * panels) * D + c0 + col) * kStepK + 8 * g) = y;
     }
   }
 }
@@ -551,19 +583,32 @@ __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
     }
 }
 
-// out = sum over the splits; rows with keep < 0 become zeros.  Four elements per thread; kShares threads, one per wave,
-// share the splits where these are many and the elements few.
+// out = sum over the splits; rows with keep < 0 become zeros.  Four elements per thread; kShares threads of a workgroup
+// share the splits where these are many and the elements few.  A launch takes two products.
+struct JoinJob {
+  const float *part;
+  int64_t part_stride;
+  int32_t splits, D;
+  int64_t rows;
+  void *out;
+  const int32_t *keep;
+  uint32_t blocks;
+};
+struct JoinJobs {
+  JoinJob job[2];
+};
+constexpr int kJoinMany = 16, kJoinShares = 8;  // splits from which eight threads share an element's
+
 template <typename T, int kShares>
-__global__ __launch_bounds__(kBlockThreads) void join_kernel(const float *part, int64_t part_stride, int32_t splits,
-                                                             T *out, int64_t rows, int32_t D, const int32_t *keep) {
+__device__ __forceinline__ void join_splits(const JoinJob &j, uint32_t block) {
   constexpr int kQuads = kBlockThreads / kShares;
   __shared__ float4 joined[kShares][kQuads];
   const int share = threadIdx.x / kQuads;
-  const int64_t total = rows * D, t = (static_cast<int64_t>(blockIdx.x) * kQuads + threadIdx.x % kQuads) * 4;
+  const int64_t total = j.rows * j.D, t = (static_cast<int64_t>(block) * kQuads + threadIdx.x % kQuads) * 4;
   float4 s{0.0f, 0.0f, 0.0f, 0.0f};
   if (t < total)
-    for (int32_t z = splits * share / kShares; z < splits * (share + 1) / kShares; ++z) {
-      const float4 x = *reinterpret_cast<const float4 *>(part + z * part_stride + t);
+    for (int32_t z = j.splits * share / kShares; z < j.splits * (share + 1) / kShares; ++z) {
+      const float4 x = *reinterpret_cast<const float4 *>(j.part + z * j.part_stride + t);
       s.x += x.x;
       s.y += x.y;
       s.z += x.z;
@@ -585,7 +630,16 @@ __global__ __launch_bounds__(kBlockThreads) void join_kernel(const float *part, 
   const float x[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (t + k < total) out[t + k] = narrow<T>(keep && keep[(t + k) / D] < 0 ? 0.0f : x[k]);
+    if (t + k < total) static_cast<T *>(j.out)[t + k] = narrow<T>(j.keep && j.keep[(t + k) / j.D] < 0 ? 0.0f : x[k]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kBlockThreads) void join_kernel(JoinJobs jobs) {
+  const bool second = blockIdx.x >= jobs.job[0].blocks;
+  const JoinJob &j = jobs.job[second];
+  const uint32_t block = second ? blockIdx.x - jobs.job[0].blocks : blockIdx.x;
+  if (j.splits >= kJoinMany) join_splits<T, kJoinShares>(j, block);
+  else join_splits<T, 1>(j, block);
 }
 
 __global__ __launch_bounds__(kBlockThreads) void zero_kernel(uint16_t *out, int64_t n) {
@@ -756,51 +810,48 @@ unsigned flat_grid(int64_t threads) {
   return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>((threads + kBlockThreads - 1) / kBlockThreads, 1 << 14)));
 }
 
-// x as an operand of the logits; float32 also leaves its rows' exponents and, with `peak`, its largest element.
+// The matrix x as an operand of the logits: used in place, or where job->out will have copied it.
 template <typename T>
-GemmOperand operand(const T *x, int64_t rows, int64_t D, const Layout &l, char *copy, int32_t *exps, uint32_t *peak,
-                    const int32_t *keep, const float *factor, hipStream_t stream) {
-  if (!l.packed) {
-    GemmOperand o;
-    o.rows = static_cast<int32_t>(rows);
-    o.p = reinterpret_cast<const uint16_t *>(x);
-    o.row = D;
-    o.step = kStepK;
-    return o;
-  }
-  auto *to = reinterpret_cast<uint16_t *>(copy);
-  if constexpr (sizeof(T) == 4)
-    split_rows_kernel<<<dim3(static_cast<unsigned>(std::min<int64_t>((rows + kWavesPerBlock - 1) / kWavesPerBlock, 4096))),
-                        dim3(kBlockThreads), 0, stream>>>(x, to, rows, static_cast<int32_t>(D), exps, peak, keep, factor);
-  else
-    pad_kernel<<<dim3(flat_grid(panel_elements(rows, D))), dim3(kBlockThreads), 0, stream>>>(
-        reinterpret_cast<const uint16_t *>(x), to, rows, static_cast<int32_t>(D));
-  return panels(to, rows, D);
+GemmOperand operand(const CopyJob &job, const Layout &l) {
+  if (l.packed) return panels(job.out, job.rows, job.D);
+  GemmOperand o;
+  o.rows = static_cast<int32_t>(job.rows);
+  o.p = static_cast<const uint16_t *>(job.x);
+  o.row = job.D;
+  o.step = kStepK;
+  return o;
 }
 
 template <typename T>
-void transpose(const T *x, const int32_t *keep, const float *factor, const uint32_t *peak, uint16_t *out, int64_t rows,
-               int64_t D, hipStream_t stream) {
+void copy_rows(CopyJobs jobs, hipStream_t stream) {
+  for (CopyJob &j : jobs.job)
+    j.blocks = j.rows == 0 ? 0
+               : sizeof(T) == 4 ? static_cast<uint32_t>(std::min<int64_t>((j.rows + kWavesPerBlock - 1) / kWavesPerBlock, 4096))
+                                : flat_grid(panel_elements(j.rows, j.D));
+  copy_rows_kernel<T><<<dim3(jobs.job[0].blocks + jobs.job[1].blocks), dim3(kBlockThreads), 0, stream>>>(jobs);
+}
+
+template <typename T>
+void copy_transposed(CopyJobs jobs, hipStream_t stream) {
   constexpr int kVec = 16 / sizeof(T);
-  const dim3 grid(static_cast<unsigned>(steps_of(rows)), static_cast<unsigned>((D + 63) / 64));
-  if (D % kVec == 0 && aligned_to(x, 16))
-    transpose_kernel<T, kVec><<<grid, dim3(kBlockThreads), 0, stream>>>(x, keep, factor, peak, out, static_cast<int32_t>(rows),
-                                                                        static_cast<int32_t>(D));
-  else
-    transpose_kernel<T, 1><<<grid, dim3(kBlockThreads), 0, stream>>>(x, keep, factor, peak, out, static_cast<int32_t>(rows),
-                                                                     static_cast<int32_t>(D));
+  bool wide = true;
+  for (CopyJob &j : jobs.job) {
+    j.blocks = static_cast<uint32_t>(steps_of(j.rows) * ((j.D + 63) / 64));
+    wide = wide && (j.rows == 0 || (j.D % kVec == 0 && aligned_to(j.x, 16)));
+  }
+  const dim3 grid(jobs.job[0].blocks + jobs.job[1].blocks);
+  if (wide) copy_transposed_kernel<T, kVec><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
+  else copy_transposed_kernel<T, 1><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
 }
 
 template <typename T>
-void join(const float *part, int64_t part_stride, int32_t splits, T *out, int64_t rows, int64_t D, const int32_t *keep,
-          hipStream_t stream) {
-  const int64_t quads = (rows * D + 3) / 4;
-  if (splits >= 16)
-    join_kernel<T, 8><<<dim3(static_cast<unsigned>((quads + 31) / 32)), dim3(kBlockThreads), 0, stream>>>(
-        part, part_stride, splits, out, rows, static_cast<int32_t>(D), keep);
-  else
-    join_kernel<T, 1><<<dim3(static_cast<unsigned>((quads + 255) / 256)), dim3(kBlockThreads), 0, stream>>>(
-        part, part_stride, splits, out, rows, static_cast<int32_t>(D), keep);
+void join(JoinJobs jobs, hipStream_t stream) {
+  for (JoinJob &j : jobs.job) {
+    const int quads = j.splits >= kJoinMany ? kBlockThreads / kJoinShares : kBlockThreads;  // of a workgroup
+    j.blocks = static_cast<uint32_t>(((j.rows * j.D + 3) / 4 + quads - 1) / quads);
+  }
+  const dim3 grid(jobs.job[0].blocks + jobs.job[1].blocks);
+  if (grid.x > 0) join_kernel<T><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
 }
 
 template <typename T, typename Id>
@@ -815,9 +866,14 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
   auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
   a.exp_a = w_exp;
   a.exp_b = h_exp;
-  a.g.b = operand(h, N, D, l, ws + l.h_pack, h_exp, nullptr, nullptr, nullptr, stream);
+  CopyJobs jobs{};
+  jobs.job[0] = CopyJob{h, reinterpret_cast<uint16_t *>(ws + l.h_pack), N, static_cast<int32_t>(D), 0, h_exp};
+  a.g.b = operand<T>(jobs.job[0], l);
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
-    a.g.a = operand(w + v0 * D, std::min(l.piece, V - v0), D, l, ws + l.w_pack, w_exp, nullptr, nullptr, nullptr, stream);
+    jobs.job[1] = CopyJob{w + v0 * D, reinterpret_cast<uint16_t *>(ws + l.w_pack), std::min(l.piece, V - v0), static_cast<int32_t>(D), 0, w_exp};
+    a.g.a = operand<T>(jobs.job[1], l);
+    if (l.packed) copy_rows<T>(jobs, stream);
+    jobs.job[0].rows = 0;  // h is there now
     a.v0 = v0;
     const int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3) {
       using Tile = decltype(tile);
@@ -865,22 +921,31 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   const float *factor = sizeof(T) == 4 ? dloss : nullptr;
   a.exp_a = w_exp;
   a.exp_b = h_exp;
-  a.g.b = operand(h, N, D, l, ws + l.h_pack, h_exp, peaks, label, factor, stream);
-  transpose(h, label, factor, peaks, ht, N, D, stream);
+  CopyJobs rows_of, transposed;
+  rows_of.job[0] = CopyJob{h, reinterpret_cast<uint16_t *>(ws + l.h_pack), N, static_cast<int32_t>(D), 0, h_exp, peaks, label, factor};
+  transposed.job[0] = rows_of.job[0];
+  transposed.job[0].out = ht;
+  a.g.b = operand<T>(rows_of.job[0], l);
   const bool dh_partial = l.dh_splits > 1 || V > l.piece;
+  JoinJobs joins{};
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
     const int64_t rows = std::min(l.piece, V - v0);
     a.v0 = static_cast<int32_t>(v0);
     a.nv_part = panel_elements(N, rows);
     a.vn_part = panel_elements(rows, N);
     uint32_t *peak = peaks ? peaks + (1 + v0 / l.piece) * kPeakSlots * kPeakStride : nullptr;
-    a.g.a = operand(w + v0 * D, rows, D, l, ws + l.w_pack, w_exp, peak, nullptr, nullptr, stream);
+    rows_of.job[1] = CopyJob{w + v0 * D, reinterpret_cast<uint16_t *>(ws + l.w_pack), rows, static_cast<int32_t>(D), 0, w_exp, peak};
+    transposed.job[1] = rows_of.job[1];
+    transposed.job[1].out = wt;
+    a.g.a = operand<T>(rows_of.job[1], l);
+    if (l.packed) copy_rows<T>(rows_of, stream);
+    copy_transposed<T>(transposed, stream);
+    rows_of.job[0].rows = transposed.job[0].rows = 0;  // h is there now
     int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3 grid) {
       using Tile = decltype(tile);
       grad_logits_kernel<Tile, T><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
-    transpose<T>(w + v0 * D, nullptr, nullptr, peak, wt, rows, D, stream);
 
     StoreArgs s{};  // dw[v, d] = sum over n of G[v, n] * h[n, d]
     s.g.steps = static_cast<int32_t>(steps_of(N));
@@ -893,7 +958,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     rc = product<T>(l.dw, s, dw + v0 * D, l.dw_splits > 1, stream);
     if (rc) return rc;
     if (l.dw_splits > 1)
-      join<T>(s.part, s.part_stride, l.dw_splits, dw + v0 * D, rows, D, nullptr, stream);
+      joins.job[0] = JoinJob{s.part, s.part_stride, l.dw_splits, static_cast<int32_t>(D), rows, dw + v0 * D, nullptr, 0};
 
     s.g.steps = static_cast<int32_t>(steps_of(rows));  // dh[n, d] = sum over v of G[n, v] * w[v, d]
     s.g.splits = l.dh_splits;
@@ -907,9 +972,10 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     s.accumulate = v0 > 0;
     rc = product<T>(l.dh, s, dh, dh_partial, stream);
     if (rc) return rc;
+    if (dh_partial && v0 + l.piece >= V)
+      joins.job[1] = JoinJob{s.part, s.part_stride, l.dh_splits, static_cast<int32_t>(D), N, dh, label, 0};
+    join<T>(joins, stream);
   }
-  if (dh_partial)
-    join<T>(reinterpret_cast<float *>(ws + l.dh_part), up(N * D, 4), l.dh_splits, dh, N, D, label, stream);
   FG_HIP_TRY(hipGetLastError());
   return FG_OK;
 }

@@ -156,7 +156,9 @@ class DenseBase:
             return time_calls(lambda: self._launch(tensors), self._ctx, num_runs)
 
     def _stream(self):
-        return torch.cuda.current_stream(self._ctx).cuda_stream
+        """hipStream_t of torch's current stream, as current_stream_handle gives it, without building a Stream object
+        (0.1 against 2 us, a quarter of a small lookup's call)."""
+        return torch._C._cuda_getCurrentRawStream(self._ctx.index)
 
     def _workspace(self, entry, *sizes):
         """A workspace of the size that the library's `entry` gives, kept by the module."""

@@ -5,8 +5,10 @@ added in float64; clipping multiplies every element by min(1, max_norm / (norm +
 shape and in type (float32, bfloat16, float16).
 """
 import bisect
+import ctypes
 import math
 
+import numpy as np
 import torch
 
 from .. import _lib
@@ -29,10 +31,13 @@ class GradNormhip(C.DenseBase):
             raise ValueError("at most %d tensors per call, got %d" % (1 << 17, len(input_placeholders)))
         types = [C.typed(p.dtype, C.ELEMENT_TYPES, "gradients") for p in input_placeholders]
         self._shapes = [torch.Size(int(s) for s in p.shape) for p in input_placeholders]
-        self._types = [t[0] for t in types]
+        self._expected = [(shape, t[0], shape.numel() * t[0].itemsize) for shape, t in zip(self._shapes, types)]
         self._list = (_lib.Tensor * max(1, len(types)))()
         for entry, shape, t in zip(self._list, self._shapes, types):
             entry.n, entry.dtype = shape.numel(), t[1]
+        # the list's address columns (data, out) as an array, so that a call sets all of them at once
+        words = np.frombuffer(self._list, dtype=np.uint64).reshape(-1, ctypes.sizeof(_lib.Tensor) // 8)
+        self._data, self._out = words[:len(types), 0], words[:len(types), 1]
         return args
 
     def _allocate(self):
@@ -41,18 +46,21 @@ class GradNormhip(C.DenseBase):
         self.out_tvm = self._norm
 
     def _checked(self, arrays):
-        if len(arrays) != len(self._shapes):
-            raise ValueError("expected %d input arrays, got %d" % (len(self._shapes), len(arrays)))
-        ctx = self._ctx
-        tensors = [as_tensor(x) for x in arrays]
-        for i, (t, shape, dtype) in enumerate(zip(tensors, self._shapes, self._types)):
+        """(tensors, their addresses) of the operands."""
+        if len(arrays) != len(self._expected):
+            raise ValueError("expected %d input arrays, got %d" % (len(self._expected), len(arrays)))
+        ctx, tensors, at = self._ctx, [], []
+        for x, (shape, dtype, _) in zip(arrays, self._expected):
+            t = x if isinstance(x, torch.Tensor) else as_tensor(x)
             if t.shape != shape or t.dtype != dtype or t.device != ctx or not t.is_contiguous():
-                C.check_typed_operand(t, shape, dtype, ctx, "gradient %d" % i)
-        return tensors
+                C.check_typed_operand(t, shape, dtype, ctx, "gradient %d" % len(tensors))
+            tensors.append(t)
+            at.append(t.data_ptr())
+        return tensors, at
 
-    def _launch(self, tensors):
-        for entry, t in zip(self._list, tensors):
-            entry.data = t.data_ptr()
+    def _launch(self, operands):
+        tensors, at = operands
+        self._data[:] = at
         _lib.check(_lib.lib().fg_grad_norm(len(tensors), self._list, self._norm.tensor.data_ptr(),
                                            self._space.data_ptr(), self._space.numel(), self._stream()))
         return self._norm
@@ -78,38 +86,33 @@ class ClipGradNormhip(GradNormhip):
         self._allocate()
         self._clipped = None
         if not self._in_place:
-            self._clipped = [NDArray(torch.zeros(s, dtype=t, device=self._ctx)) for s, t in zip(self._shapes, self._types)]
-            for entry, out in zip(self._list, self._clipped):
-                entry.out = out.tensor.data_ptr()
-            spans = sorted((c.tensor.data_ptr(), c.tensor.numel() * c.tensor.element_size())
-                           for c in self._clipped if c.tensor.numel())
+            self._clipped = [NDArray(torch.zeros(shape, dtype=t, device=self._ctx)) for shape, t, _ in self._expected]
+            self._out[:] = [c.tensor.data_ptr() for c in self._clipped]
+            spans = sorted((c.tensor.data_ptr(), size) for c, (_, _, size) in zip(self._clipped, self._expected) if size)
             self._out_begin, self._out_end = [b for b, _ in spans], [b + n for b, n in spans]
         self._built = True
 
     def _checked(self, arrays):
-        tensors = super()._checked(arrays)
+        tensors, at = super()._checked(arrays)
         if self._in_place:
-            spans, end = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel()), 0
-            for begin, size in spans:
+            end = 0
+            for begin, size in sorted((b, size) for b, (_, _, size) in zip(at, self._expected) if size):
                 if begin < end:
                     raise ValueError("the gradients overlap each other")
                 end = begin + size
-            return tensors
-        for t in tensors:
-            if t.numel():
-                begin = t.data_ptr()
-                i = bisect.bisect_left(self._out_begin, begin + t.numel() * t.element_size()) - 1
-                if i >= 0 and self._out_end[i] > begin:      # the outputs are disjoint: the last one that starts below
-                    raise ValueError("a gradient overlaps the module's outputs")
-        return tensors
-
-    def _launch(self, tensors):
-        if self._in_place:
-            for entry, t in zip(self._list, tensors):
-                entry.data = entry.out = t.data_ptr()
         else:
-            for entry, t in zip(self._list, tensors):
-                entry.data = t.data_ptr()
+            begins, ends = self._out_begin, self._out_end
+            for begin, (_, _, size) in zip(at, self._expected):
+                i = bisect.bisect_left(begins, begin + size) - 1
+                if size and i >= 0 and ends[i] > begin:      # the outputs are disjoint: the last one that starts below
+                    raise ValueError("a gradient overlaps the module's outputs")
+        return tensors, at
+
+    def _launch(self, operands):
+        tensors, at = operands
+        self._data[:] = at
+        if self._in_place:
+            self._out[:] = at
         _lib.check(_lib.lib().fg_grad_clip(len(tensors), self._list, self._max_norm, self._eps,
                                            self._norm.tensor.data_ptr(), self._space.data_ptr(), self._space.numel(),
                                            self._stream()))
