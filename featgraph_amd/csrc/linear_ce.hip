@@ -7,10 +7,10 @@
 //
 // Forward: one matrix product whose epilogue keeps, per row n and tile of vocabulary, the largest logit and the sum
 // of exponentials relative to it; a second kernel joins the tiles and takes the label's logit as a dot product of its
-// own.  Backward: the logits are computed again piece by piece of the vocabulary; the epilogue turns them into P,
-// written once as [n, v] and once as [v, n], and two more products over them give the piece's rows of dw and its
-// share of dh.  All three products are the same kernel over operands with k contiguous, so h and w are transposed
-// into copies for the backward products (2 N D + 2 V D elements of traffic against 6 N V D flops).
+// own.  Backward: the logits are computed again piece by piece of the vocabulary; the epilogue turns them into P, and two
+// more products over P give the piece's rows of dw and its share of dh.  P is stored once, as [v, n]: dw's product reads
+// its rows, dh's its columns (mfma_gemm.hpp).  h and w are transposed into copies for these products (2 N D + 2 V D
+// elements of traffic against 6 N V D flops).
 //
 // Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step of each
 // term, random in sign; the results are rounded to bfloat16 themselves); everything between is float32.  float32
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
     sum[j] = 0.0f;
     label[j] = n < a.g.b.rows ? static_cast<int64_t>(static_cast<const Id *>(a.labels)[n]) - a.v0 - first_v : -1;
   }
-  gemm_tiles<Tile, T>(a.g, at, tiles, lds, acc, [&](int tile) {
+  gemm_tiles<Tile, T, false>(a.g, at, tiles, lds, acc, [&](int tile) {
     const int64_t v0 = first_v + static_cast<int64_t>(tile) * Tile::BM;
     to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
 #pragma unroll
@@ -398,13 +398,11 @@ struct GradArgs {
   const int32_t *label;      // [N], negative: ignored
   const float *lse, *dloss;  // [N]
   int32_t v0;                // first vocabulary row of the piece
-  uint16_t *nv, *vn;         // P as panels of [n, v] and of [v, n], parts apart by *_part
-  int64_t nv_part, vn_part;
+  uint16_t *vn;              // P as panels of [v, n], the rows of the piece padded to whole panels with zeros
+  int64_t vn_part;           // elements from one part to the next
 };
 
-// T: type of the operands, which says how P is stored.  The [v, n] copy is written from the registers, four n per lane;
-// the [n, v] copy goes through LDS, so that its rows leave in 16-byte pieces that follow each other (a 16-byte piece of
-// row n lies at piece ^ n within the row, so that neither side meets bank conflicts).
+// T: type of the operands, which says how P is stored: straight from the registers, four n per lane.
 template <typename Tile, typename T>
 __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
@@ -452,8 +450,6 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
           if (32 * i + acc_row(k, 0) >= end) acc.c[i][j][k] = 0.0f;
     }
   }
-  constexpr int kPieces = Tile::BM / 8;  // of 16 bytes in a row of the [n, v] tile
-  auto place = [](int n, int piece) { return piece ^ (kPieces == 8 ? (n >> 1) & 7 : n & (kPieces - 1)); };
   // the 16-bit form of the accumulator x; a float32's rest takes its place for the next part
   auto take = [](float &x) -> uint32_t {
     const uint32_t bits = part_of<T>(x, 0);
@@ -463,22 +459,19 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
     }
     return bits;
   };
-  const int64_t first_n = static_cast<int64_t>(at.tn) * Tile::BN;
-  const int first_v = at.tm * Tile::BM;
   const int64_t M = a.g.a.rows, N = a.g.b.rows;
   const int64_t end_v = (M + kStepK - 1) / kStepK * kStepK, end_n = (N + kStepK - 1) / kStepK * kStepK;  // of the panels
-  const bool whole = first_v + Tile::BM <= M && first_n + Tile::BN <= N;
+  const bool whole = static_cast<int64_t>(at.tm + 1) * Tile::BM <= M && static_cast<int64_t>(at.tn + 1) * Tile::BN <= N;
   auto store = [&](auto inside, int part) {  // inside: the whole tile lies within the matrix
     constexpr bool kInside = decltype(inside)::value;
 #pragma unroll
     for (int j = 0; j < Tile::TN; ++j) {
       const int64_t col = n0 + 32 * j + lane % 32 / 4 * 4;
-      const int n = wave_n + 32 * j + lane % 32;
 #pragma unroll
       for (int i = 0; i < Tile::TM; ++i) {
         FG_IN_ORDER();
         const int64_t row = v0 + 32 * i + acc_row(0, lane) + lane % 4;
-        uint16_t *to = a.vn + part * a.vn_part + panel_at(M, row, col);
+        uint16_t *to = a.vn + part * a.vn_part + panel_at(end_v, row, col);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float e[4] = {acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
@@ -489,25 +482,14 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
           x.y |= take(e[3]) << 16;
 #pragma unroll
           for (int k = 0; k < 4; ++k) acc.c[i][j][4 * q + k] = e[k];
-          const int v = wave_v + 32 * i + 8 * q;  // lanes 32..63: the second half of the piece
-          *reinterpret_cast<uint2 *>(lds + n * Tile::BM + place(n, v / 8) * 8 + lane / 32 * 4) = x;
           const uint2 y = turn4(x, lane);
-          if (kInside || (row + 8 * q < M && col < end_n)) *reinterpret_cast<uint2 *>(to + 8 * q * kStepK) = y;
+          if (kInside || (row + 8 * q < end_v && col < end_n)) *reinterpret_cast<uint2 *>(to + 8 * q * kStepK) = y;
         }
       }
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int t = threadIdx.x; t < Tile::BN * kPieces; t += Tile::kThreads) {  // panel by panel, eight pieces per row
-      const int piece = t / (8 * Tile::BN) * 8 + t % 8, n = t / 8 % Tile::BN;
-      if (kInside || (first_n + n < N && first_v + piece * 8 < end_v))
-        *reinterpret_cast<uint4 *>(a.nv + part * a.nv_part + panel_at(N, first_n + n, first_v + piece * 8)) =
-            *reinterpret_cast<const uint4 *>(lds + n * Tile::BM + place(n, piece) * 8);
     }
   };
 #pragma unroll
   for (int part = 0; part < Multiply<T>::kParts; ++part) {
-    if (part) __syncthreads();  // the first part is no longer read
     if (sizeof(T) == 2 && whole) store(std::true_type{}, part);  // a second copy of the code costs float32 its registers
     else store(std::false_type{}, part);
   }
@@ -525,13 +507,13 @@ struct StoreArgs {
   int32_t wide;            // 16-bit out: four elements per store (its alignment and the row length allow it)
 };
 
-// kPartial: the sums go to a.part for join_kernel, else rounded to a.out.
-template <typename Tile, typename T, bool kPartial>
+// kPartial: the sums go to a.part for join_kernel, else rounded to a.out.  kTurnA: operand a is turned.
+template <typename Tile, typename T, bool kPartial, bool kTurnA>
 __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
   const GemmPlace at = gemm_place(a.g);
-  gemm_tile<Tile, T>(a.g, at, lds, acc);
+  gemm_tile<Tile, T, kTurnA>(a.g, at, lds, acc);
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
   const int64_t m0 = static_cast<int64_t>(at.tm) * Tile::BM + wm * (Tile::BM / Tile::WM);
@@ -543,7 +525,7 @@ __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
       for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int64_t m = m0 + 32 * i + acc_row(4 * q, lane) + lane % 4;
+          const int64_t m = m0 + tile_row<Tile, kTurnA>(i, acc_row(4 * q, lane) + lane % 4);
           const bool zero = m < M && a.keep && a.keep[m] < 0;
 #pragma unroll
           for (int j = 0; j < Tile::TN; ++j) {
@@ -564,7 +546,7 @@ __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
   for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int64_t m = m0 + 32 * i + acc_row(r, lane);
+      const int64_t m = m0 + tile_row<Tile, kTurnA>(i, acc_row(r, lane));
       if (m >= M) continue;
       const bool zero = !kPartial && a.keep && a.keep[m] < 0;
       const float f = sizeof(T) == 4 && a.factor ? a.factor[m] : 1.0f;
@@ -733,7 +715,7 @@ struct Layout {
   int64_t piece;         // vocabulary rows per piece, a multiple of 256
   TileKind logits, dh, dw;
   int dh_splits, dw_splits;
-  int64_t h_pack, w_pack, h_exp, w_exp, peaks, stats, label, ht, wt, nv, vn, dh_part, dw_part, bytes;
+  int64_t h_pack, w_pack, h_exp, w_exp, peaks, stats, label, ht, wt, vn, dh_part, dw_part, bytes;
 };
 
 Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool backward) {
@@ -742,8 +724,9 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   l.segments = dtype == FG_F32 ? kSegments : 1;
   l.packed = dtype == FG_F32 || D % kStepK != 0 || !aligned;
   int64_t per_row = l.packed ? 2 * l.parts * up(D, kStepK) : 0;
-  if (backward) per_row += 2 * l.parts * (N + up(N, kStepK) + D);
-  const int64_t most = per_row ? std::max<int64_t>(256, kPieceBytes / per_row / 256 * 256) : up(V, 256);
+  if (backward) per_row += 2 * l.parts * (up(N, kStepK) + D);
+  // at most 2^22 rows, which 32-bit offsets into four panels reach
+  const int64_t most = per_row ? std::clamp<int64_t>(kPieceBytes / per_row / 256 * 256, 256, 1 << 22) : up(V, 256);
   l.piece = up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), 256);  // as many pieces as needed, of equal size
   if (const int64_t rows = config().ce_piece_rows) l.piece = up(rows, 256);
   const int64_t in_piece = std::min(l.piece, V);
@@ -779,8 +762,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
     l.label = take(4 * N);
     l.ht = take(2 * l.parts * panel_elements(D, N));
     l.wt = take(2 * l.parts * panel_elements(D, in_piece));
-    l.nv = take(2 * l.parts * panel_elements(N, in_piece));
-    l.vn = take(2 * l.parts * panel_elements(in_piece, N));
+    l.vn = take(2 * l.parts * panel_elements(up(in_piece, kStepK), N));
     l.dh_part = take(l.dh_splits > 1 || V > l.piece ? 4 * l.dh_splits * up(N * D, 4) : 0);
     l.dw_part = take(l.dw_splits > 1 ? 4 * l.dw_splits * up(in_piece * D, 4) : 0);
   }
@@ -890,16 +872,16 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
 }
 
 // out[M, D] = the product, through partial sums where k is shared or earlier pieces have added to them
-template <typename T>
+template <typename T, bool kTurnA>
 int product(TileKind kind, StoreArgs a, T *out, bool partial, hipStream_t stream) {
   a.out = out;
   a.wide = a.g.b.rows % 4 == 0 && aligned_to(out, 8);
   return with_tile(kind, &a.g, [&](auto tile, dim3 grid) {
     using Tile = decltype(tile);
     if (partial)
-      product_kernel<Tile, T, true><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
+      product_kernel<Tile, T, true, kTurnA><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
     else
-      product_kernel<Tile, T, false><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
+      product_kernel<Tile, T, false, kTurnA><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
   });
 }
 
@@ -908,12 +890,11 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
              T *dw, char *ws, const Layout &l, hipStream_t stream) {
   const int32_t *label = reinterpret_cast<const int32_t *>(ws + l.label);
   auto *ht = reinterpret_cast<uint16_t *>(ws + l.ht), *wt = reinterpret_cast<uint16_t *>(ws + l.wt);
-  auto *nv = reinterpret_cast<uint16_t *>(ws + l.nv), *vn = reinterpret_cast<uint16_t *>(ws + l.vn);
+  auto *vn = reinterpret_cast<uint16_t *>(ws + l.vn);
   GradArgs a{};
   a.label = label;
   a.lse = lse;
   a.dloss = dloss;
-  a.nv = nv;
   a.vn = vn;
   a.g.steps = static_cast<int32_t>(steps_of(D));
   auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
@@ -931,8 +912,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   for (int64_t v0 = 0; v0 < V; v0 += l.piece) {
     const int64_t rows = std::min(l.piece, V - v0);
     a.v0 = static_cast<int32_t>(v0);
-    a.nv_part = panel_elements(N, rows);
-    a.vn_part = panel_elements(rows, N);
+    a.vn_part = panel_elements(up(rows, kStepK), N);
     uint32_t *peak = peaks ? peaks + (1 + v0 / l.piece) * kPeakSlots * kPeakStride : nullptr;
     rows_of.job[1] = CopyJob{w + v0 * D, reinterpret_cast<uint16_t *>(ws + l.w_pack), rows, static_cast<int32_t>(D), 0, w_exp, peak};
     transposed.job[1] = rows_of.job[1];
@@ -950,19 +930,20 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     StoreArgs s{};  // dw[v, d] = sum over n of G[v, n] * h[n, d]
     s.g.steps = static_cast<int32_t>(steps_of(N));
     s.g.splits = l.dw_splits;
-    s.g.a = panels(vn, rows, N);
+    s.g.a = panels(vn, up(rows, kStepK), N);
+    s.g.a.rows = static_cast<int32_t>(rows);
     s.g.b = panels(ht, D, N);
     s.peak = peaks;
     s.part = reinterpret_cast<float *>(ws + l.dw_part);
     s.part_stride = up(rows * D, 4);
-    rc = product<T>(l.dw, s, dw + v0 * D, l.dw_splits > 1, stream);
+    rc = product<T, false>(l.dw, s, dw + v0 * D, l.dw_splits > 1, stream);
     if (rc) return rc;
     if (l.dw_splits > 1)
       joins.job[0] = JoinJob{s.part, s.part_stride, l.dw_splits, static_cast<int32_t>(D), rows, dw + v0 * D, nullptr, 0};
 
     s.g.steps = static_cast<int32_t>(steps_of(rows));  // dh[n, d] = sum over v of G[n, v] * w[v, d]
     s.g.splits = l.dh_splits;
-    s.g.a = panels(nv, N, rows);
+    s.g.a = turned_panels(vn, N, rows);
     s.g.b = panels(wt, D, rows);
     s.keep = label;
     s.factor = factor;
@@ -970,7 +951,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     s.part = reinterpret_cast<float *>(ws + l.dh_part);
     s.part_stride = up(N * D, 4);
     s.accumulate = v0 > 0;
-    rc = product<T>(l.dh, s, dh, dh_partial, stream);
+    rc = product<T, true>(l.dh, s, dh, dh_partial, stream);
     if (rc) return rc;
     if (dh_partial && v0 + l.piece >= V)
       joins.job[1] = JoinJob{s.part, s.part_stride, l.dh_splits, static_cast<int32_t>(D), N, dh, label, 0};

@@ -16,6 +16,10 @@
 // take the same piece of consecutive rows, spread over all banks.  The permutation is applied on the way in, by what
 // each lane fetches.  Rows past the operands' ends are read as the last row and dropped by the epilogues; k is a
 // multiple of 64 (padded copies hold zeros there).
+//
+// A may also be turned: panels of 64 of its rows, one line per k.  Its stage is then [64 k][BM] in LDS, and a lane reads
+// TM neighbouring rows of eight k lines; halves of two lines put together are a pair of k of one row.  The TM rows belong
+// to the TM blocks of the wave, so that nothing moves between lanes: row r of block i is row TM * r + i of the wave's.
 #pragma once
 
 #include <type_traits>
@@ -77,6 +81,17 @@ inline GemmOperand panels(const uint16_t *p, int64_t rows, int64_t k) {
   o.rows = static_cast<int32_t>(rows);
   return o;
 }
+// Rows of the same panels as columns, and columns as rows: `rows` operand rows over `k` k lines, padded to whole panels.
+inline GemmOperand turned_panels(const uint16_t *p, int64_t rows, int64_t k) {
+  const int64_t lines = (k + kStepK - 1) / kStepK * kStepK;
+  GemmOperand o;
+  o.p = p;
+  o.part = panel_elements(lines, rows);
+  o.row = lines;  // a panel of 64 rows has `lines` lines of 64
+  o.step = kStepK * kStepK;
+  o.rows = static_cast<int32_t>(rows);
+  return o;
+}
 __device__ __forceinline__ int64_t panel_at(int64_t rows, int64_t row, int64_t k) {
   return k / kStepK * (rows * kStepK) + row * kStepK + k % kStepK;
 }
@@ -123,6 +138,12 @@ __device__ __forceinline__ GemmPlace gemm_place(const GemmShape &g) {
   return p;
 }
 
+// Row of a wave's rows that register r of block i holds.
+template <typename Tile, bool kTurnA>
+__device__ __forceinline__ int tile_row(int i, int acc_row) {
+  return kTurnA ? Tile::TM * acc_row + i : 32 * i + acc_row;
+}
+
 template <typename Tile>
 struct GemmAcc {
   f32x16 c[Tile::TM][Tile::TN];
@@ -152,7 +173,7 @@ __device__ __forceinline__ void clear(GemmAcc<Tile> &acc) {
       for (int r = 0; r < 16; ++r) acc.c[i][j][r] = 0.0f;
 }
 
-template <typename Tile, typename T, typename Done>
+template <typename Tile, typename T, bool kTurnA, typename Done>
 __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &at, int tiles, uint16_t *lds,
                                            GemmAcc<Tile> &acc, Done &&done) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass lacks the loads to LDS
@@ -170,8 +191,14 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
   uint32_t off_a[Tile::kLoadsA], off_b[Tile::kLoadsB];
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsA; ++j) {
-    const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
-    off_a[j] = row * pitch_a + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
+    if constexpr (kTurnA) {
+      constexpr int kLine = Tile::BM / 8;  // 16-byte pieces of a k line in LDS
+      const int at_piece = (wave + j * Tile::kWaves) * kWaveSize + lane, k = at_piece / kLine, piece = at_piece % kLine;
+      off_a[j] = static_cast<uint32_t>(piece / 8) * (static_cast<uint32_t>(g.a.row) * (kStepK * 2)) + k * (kStepK * 2) + piece % 8 * 16;
+    } else {
+      const int row = (wave + j * Tile::kWaves) * 8 + lane / 8;
+      off_a[j] = row * pitch_a + ((lane % 8) ^ ((row >> 1) & 7)) * 16;
+    }
   }
 #pragma unroll
   for (int j = 0; j < Tile::kLoadsB; ++j) {
@@ -188,16 +215,21 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
   // always the same number of them under way.
   struct Cursor {
     const uint16_t *p;
-    int bytes, seg, slot, left, tile_left, until;  // until: steps before p has to be taken anew
+    uint32_t bytes;
+    int seg, slot, left, tile_left, until;  // until: steps before p has to be taken anew
   };
   const int first_seg = first / g.steps, first_step = first - first_seg * g.steps;
   int64_t m_a = m0;  // first row of the tile that cursor a is in
-  auto begin = [&](Cursor &c, const GemmOperand &o, int64_t row, int rows, int step, int hi_segment) {
+  auto begin = [&](Cursor &c, const GemmOperand &o, int64_t row, int rows, int step, int hi_segment, auto turned) {
     c.p = o.p + (M::kSegments == 3 && c.seg == hi_segment ? o.part : 0) + row * o.row + step * o.step;
-    c.bytes = static_cast<int>(min<int64_t>(rows, o.rows - row) - 1) * static_cast<int>(o.row * 2) + kStepK * 2;
+    const uint32_t there = static_cast<uint32_t>(min<int64_t>(rows, o.rows - row));
+    if constexpr (decltype(turned)::value)
+      c.bytes = ((there + kStepK - 1) / kStepK - 1) * (static_cast<uint32_t>(o.row) * (kStepK * 2)) + kStepK * kStepK * 2;
+    else
+      c.bytes = (there - 1) * static_cast<uint32_t>(o.row * 2) + kStepK * 2;
     c.until = min(g.steps - step, c.tile_left);
   };
-  auto advance = [&](Cursor &c, const GemmOperand &o, int64_t &row, int rows, int stride, int hi_segment, int stages) {
+  auto advance = [&](Cursor &c, const GemmOperand &o, int64_t &row, int rows, int stride, int hi_segment, int stages, auto turned) {
     if (++c.slot == stages) c.slot = 0;
     c.p += o.step;
     --c.tile_left;
@@ -212,15 +244,16 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
         step = first_step;
         row += stride;
       }
-      begin(c, o, row, rows, step, hi_segment);
+      begin(c, o, row, rows, step, hi_segment, turned);
     }
   };
   Cursor ca{nullptr, 0, first_seg, 0, n, per_tile, 0}, cb = ca;
+  using TurnA = std::integral_constant<bool, kTurnA>;
   int64_t m_b = n0;
-  begin(ca, g.a, m_a, Tile::BM, first_step, 1);
-  begin(cb, g.b, m_b, Tile::BN, first_step, 0);
-  auto advance_a = [&]() { advance(ca, g.a, m_a, Tile::BM, Tile::BM, 1, Tile::kStagesA); };
-  auto advance_b = [&]() { advance(cb, g.b, m_b, Tile::BN, 0, 0, 2); };
+  begin(ca, g.a, m_a, Tile::BM, first_step, 1, TurnA{});
+  begin(cb, g.b, m_b, Tile::BN, first_step, 0, std::false_type{});
+  auto advance_a = [&]() { advance(ca, g.a, m_a, Tile::BM, Tile::BM, 1, Tile::kStagesA, TurnA{}); };
+  auto advance_b = [&]() { advance(cb, g.b, m_b, Tile::BN, 0, 0, 2, std::false_type{}); };
   uint16_t *const lds_b = lds + Tile::kStagesA * Tile::kStageA;
   auto load_a = [&](int j) {
     const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(ca.p), 0, ca.bytes, 0x00020000);
@@ -248,15 +281,27 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
   const int row_a = wm * (Tile::BM / Tile::WM) + lane % 32, row_b = wn * (Tile::BN / Tile::WN) + lane % 32;
   const int at_a = row_a * kStepK, at_b = row_b * kStepK;
   const int twist = (lane >> 1) & 7;
+  // turned: k lines 16 * quarter + 8 * (l / 32) on, rows TM * (l % 32) on
+  static_assert(Tile::TM == 2 || Tile::TM == 4, "a turned row group is one or two words");
+  typedef uint32_t Rows __attribute__((ext_vector_type(Tile::TM / 2)));
+  const int at_turned = 8 * (lane / 32) * Tile::BM + wm * (Tile::BM / Tile::WM) + lane % 32 * Tile::TM;
   struct Fragments {
-    bf16x8 a[Tile::TM], b[Tile::TN];
+    bf16x8 a[kTurnA ? 1 : Tile::TM], b[Tile::TN];
+    Rows lines[kTurnA ? 8 : 1];
   };
   int slot_a = 0, slot_b = 0;  // of the step that is read
   auto read = [&](Fragments &f, int quarter) {
     const int piece = ((2 * quarter + lane / 32) ^ twist) * 8;
-    const uint16_t *sa = lds + slot_a * Tile::kStageA + at_a + piece, *sb = lds_b + slot_b * Tile::kStageB + at_b + piece;
+    const uint16_t *sb = lds_b + slot_b * Tile::kStageB + at_b + piece;
+    if constexpr (kTurnA) {
+      const uint16_t *sa = lds + slot_a * Tile::kStageA + quarter * 16 * Tile::BM + at_turned;
 #pragma unroll
-    for (int t = 0; t < Tile::TM; ++t) f.a[t] = *reinterpret_cast<const bf16x8 *>(sa + t * 32 * kStepK);
+      for (int k = 0; k < 8; ++k) f.lines[k] = *reinterpret_cast<const Rows *>(sa + k * Tile::BM);
+    } else {
+      const uint16_t *sa = lds + slot_a * Tile::kStageA + at_a + piece;
+#pragma unroll
+      for (int t = 0; t < Tile::TM; ++t) f.a[t] = *reinterpret_cast<const bf16x8 *>(sa + t * 32 * kStepK);
+    }
 #pragma unroll
     for (int t = 0; t < Tile::TN; ++t) f.b[t] = *reinterpret_cast<const bf16x8 *>(sb + t * 32 * kStepK);
   };
@@ -265,10 +310,23 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     constexpr int kQuarter = decltype(quarter)::value, kProducts = Tile::TM * Tile::TN;
     constexpr int kShare = kQuarter < kQuarters ? kPerQuarter : 0;
     __builtin_amdgcn_sched_barrier(0);  // the reads before it are under way
+    bf16x8 row;
 #pragma unroll
     for (int p = 0; p < kProducts; ++p) {
       const int t = p / Tile::TN, u = p % Tile::TN;
-      acc.c[t][u] = M::mfma(f.a[t], f.b[u], acc.c[t][u]);
+      if constexpr (kTurnA) {
+        if (u == 0) {
+          typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+          u32x4 w;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            w[k] = __builtin_amdgcn_perm(f.lines[2 * k + 1][t / 2], f.lines[2 * k][t / 2], t % 2 ? 0x07060302u : 0x05040100u);
+          row = __builtin_bit_cast(bf16x8, w);
+        }
+      } else {
+        row = f.a[t];
+      }
+      acc.c[t][u] = M::mfma(row, f.b[u], acc.c[t][u]);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int l = kShare * p / kProducts; l < kShare * (p + 1) / kProducts; ++l) load_one(kQuarter * kPerQuarter + l);
@@ -332,9 +390,9 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
 }
 
 // One tile, left in acc.
-template <typename Tile, typename T>
+template <typename Tile, typename T, bool kTurnA = false>
 __device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &at, uint16_t *lds, GemmAcc<Tile> &acc) {
-  gemm_tiles<Tile, T>(g, at, 1, lds, acc, [](int) {});
+  gemm_tiles<Tile, T, kTurnA>(g, at, 1, lds, acc, [](int) {});
 }
 
 }  // namespace fg
