@@ -265,18 +265,25 @@ __device__ __forceinline__ void to_logits(GemmAcc<Tile> &acc, const int32_t *exp
   }
 }
 
+// First tile of a workgroup that takes one tile of rows n and a range of the vocabulary, and how many follow each other.
+__device__ __forceinline__ GemmPlace range_place(const GemmShape &g, int ranges, int *range, int *tiles) {
+  GemmShape places = g;
+  places.tiles_m = ranges;
+  GemmPlace at = gemm_place(places);
+  *range = at.tm;
+  at.tm = static_cast<int32_t>(static_cast<int64_t>(g.tiles_m) * *range / ranges);
+  *tiles = static_cast<int>(static_cast<int64_t>(g.tiles_m) * (*range + 1) / ranges) - at.tm;
+  return at;
+}
+
 // A workgroup takes one tile of rows n and a range of the vocabulary, tile after tile without a pause in its loads; each
 // lane keeps the statistics of the logits it meets (its column n, half the rows of its wave) until the end.
 template <typename Tile, typename T, typename Id>
 __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
-  GemmShape places = a.g;
-  places.tiles_m = a.ranges;
-  GemmPlace at = gemm_place(places);
-  const int range = at.tm;
-  at.tm = static_cast<int32_t>(static_cast<int64_t>(a.g.tiles_m) * range / a.ranges);
-  const int tiles = static_cast<int>(static_cast<int64_t>(a.g.tiles_m) * (range + 1) / a.ranges) - at.tm;
+  int range, tiles;
+  const GemmPlace at = range_place(a.g, a.ranges, &range, &tiles);
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
   const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wn * (Tile::BN / Tile::WN);
@@ -398,6 +405,7 @@ struct GradArgs {
   const int32_t *label;      // [N], negative: ignored
   const float *lse, *dloss;  // [N]
   int32_t v0;                // first vocabulary row of the piece
+  int32_t ranges;            // that the tiles of vocabulary are divided into
   uint16_t *vn;              // P as panels of [v, n], the rows of the piece padded to whole panels with zeros
   int64_t vn_part;           // elements from one part to the next
 };
@@ -407,49 +415,27 @@ template <typename Tile, typename T>
 __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
-  const GemmPlace at = gemm_place(a.g);
-  gemm_tile<Tile, T>(a.g, at, lds, acc);
+  int range, tiles;
+  const GemmPlace at = range_place(a.g, a.ranges, &range, &tiles);
   const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
-  const int wave_v = wm * (Tile::BM / Tile::WM), wave_n = wn * (Tile::BN / Tile::WN);
-  const int v0 = at.tm * Tile::BM + wave_v;
-  const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wave_n;
-  to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
+  const int first_v = at.tm * Tile::BM + wm * (Tile::BM / Tile::WM);
+  const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wn * (Tile::BN / Tile::WN);
   // P = exp2(l * log2(e) - r) * 2^(r - lse * log2(e)) with a whole r: the first factor is one multiply-add, rounded once,
   // the second one is taken per row, in double, together with what P is stored times.
+  int32_t label[Tile::TN];
+  float whole_lse[Tile::TN], times[Tile::TN], scale[Tile::TN];
 #pragma unroll
   for (int j = 0; j < Tile::TN; ++j) {
     const int64_t n = n0 + 32 * j + lane % 32;
-    const int32_t label = n < a.g.b.rows ? a.label[n] : -1;
-    const float times = label < 0 ? 0.0f : sizeof(T) == 4 ? static_cast<float>(1 << kTop) : a.dloss[n];
-    const double lse2 = label < 0 ? 0.0 : static_cast<double>(a.lse[n]) * 1.44269504088896340736;
-    const float r = static_cast<float>(rint(lse2));
-    const float scale = times * __builtin_amdgcn_exp2f(static_cast<float>(static_cast<double>(r) - lse2));
-    const int32_t hit = label >= 0 ? label - a.v0 - v0 : -1;  // row of this wave's block that is the label's
-#pragma unroll
-    for (int i = 0; i < Tile::TM; ++i)
-#pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][k], kLog2e, -r)) * scale;
-        acc.c[i][j][k] = label >= 0 ? p : 0.0f;
-      }
-    if (__any(hit >= 0 && hit < Tile::BM / Tile::WM)) {
-      const int mine = hit - acc_row(0, lane);
-#pragma unroll
-      for (int i = 0; i < Tile::TM; ++i)
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (32 * i + acc_row(k, 0) == mine) acc.c[i][j][k] -= times;
-    }
-    if (v0 + Tile::BM / Tile::WM > a.g.a.rows) {  // nothing past the end
-      const int end = max(a.g.a.rows - v0, 0) - acc_row(0, lane);
-#pragma unroll
-      for (int i = 0; i < Tile::TM; ++i)
-#pragma unroll
-        for (int k = 0; k < 16; ++k)
-          if (32 * i + acc_row(k, 0) >= end) acc.c[i][j][k] = 0.0f;
-    }
+    label[j] = n < a.g.b.rows ? a.label[n] : -1;
+    times[j] = label[j] < 0 ? 0.0f : sizeof(T) == 4 ? static_cast<float>(1 << kTop) : a.dloss[n];
+    const double lse2 = label[j] < 0 ? 0.0 : static_cast<double>(a.lse[n]) * 1.44269504088896340736;
+    whole_lse[j] = static_cast<float>(rint(lse2));
+    scale[j] = times[j] * __builtin_amdgcn_exp2f(static_cast<float>(static_cast<double>(whole_lse[j]) - lse2));
   }
+  const int64_t M = a.g.a.rows, N = a.g.b.rows;
+  const int64_t end_v = (M + kStepK - 1) / kStepK * kStepK, end_n = (N + kStepK - 1) / kStepK * kStepK;  // of the panels
   // the 16-bit form of the accumulator x; a float32's rest takes its place for the next part
   auto take = [](float &x) -> uint32_t {
     const uint32_t bits = part_of<T>(x, 0);
@@ -459,40 +445,70 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
     }
     return bits;
   };
-  const int64_t M = a.g.a.rows, N = a.g.b.rows;
-  const int64_t end_v = (M + kStepK - 1) / kStepK * kStepK, end_n = (N + kStepK - 1) / kStepK * kStepK;  // of the panels
-  const bool whole = static_cast<int64_t>(at.tm + 1) * Tile::BM <= M && static_cast<int64_t>(at.tn + 1) * Tile::BN <= N;
-  auto store = [&](auto inside, int part) {  // inside: the whole tile lies within the matrix
-    constexpr bool kInside = decltype(inside)::value;
+  gemm_tiles<Tile, T, false>(a.g, at, tiles, lds, acc, [&](int tile) {
+    const int v0 = first_v + tile * Tile::BM;
+    to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
 #pragma unroll
     for (int j = 0; j < Tile::TN; ++j) {
-      const int64_t col = n0 + 32 * j + lane % 32 / 4 * 4;
 #pragma unroll
-      for (int i = 0; i < Tile::TM; ++i) {
-        FG_IN_ORDER();
-        const int64_t row = v0 + 32 * i + acc_row(0, lane) + lane % 4;
-        uint16_t *to = a.vn + part * a.vn_part + panel_at(end_v, row, col);
+      for (int i = 0; i < Tile::TM; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float e[4] = {acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
-          uint2 x;
-          x.x = take(e[0]);
-          x.x |= take(e[1]) << 16;
-          x.y = take(e[2]);
-          x.y |= take(e[3]) << 16;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc.c[i][j][4 * q + k] = e[k];
-          const uint2 y = turn4(x, lane);
-          if (kInside || (row + 8 * q < end_v && col < end_n)) *reinterpret_cast<uint2 *>(to + 8 * q * kStepK) = y;
+        for (int k = 0; k < 16; ++k) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][k], kLog2e, -whole_lse[j])) * scale[j];
+          acc.c[i][j][k] = label[j] >= 0 ? p : 0.0f;
         }
+      const int32_t hit = label[j] >= 0 ? label[j] - a.v0 - v0 : -1;  // row of this wave's block that is the label's
+      if (__any(hit >= 0 && hit < Tile::BM / Tile::WM)) {
+        const int mine = hit - acc_row(0, lane);
+#pragma unroll
+        for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (32 * i + acc_row(k, 0) == mine) acc.c[i][j][k] -= times[j];
+      }
+      if (v0 + Tile::BM / Tile::WM > M) {  // nothing past the end
+        const int end = max(static_cast<int>(M) - v0, 0) - acc_row(0, lane);
+#pragma unroll
+        for (int i = 0; i < Tile::TM; ++i)
+#pragma unroll
+          for (int k = 0; k < 16; ++k)
+            if (32 * i + acc_row(k, 0) >= end) acc.c[i][j][k] = 0.0f;
       }
     }
-  };
+    const bool whole = v0 + Tile::BM / Tile::WM <= M && n0 + Tile::BN / Tile::WN <= N;
+    auto store = [&](auto inside, int part) {  // inside: the wave's whole block lies within the matrix
+      constexpr bool kInside = decltype(inside)::value;
 #pragma unroll
-  for (int part = 0; part < Multiply<T>::kParts; ++part) {
-    if (sizeof(T) == 2 && whole) store(std::true_type{}, part);  // a second copy of the code costs float32 its registers
-    else store(std::false_type{}, part);
-  }
+      for (int j = 0; j < Tile::TN; ++j) {
+        const int64_t col = n0 + 32 * j + lane % 32 / 4 * 4;
+#pragma unroll
+        for (int i = 0; i < Tile::TM; ++i) {
+          FG_IN_ORDER();
+          const int64_t row = v0 + 32 * i + acc_row(0, lane) + lane % 4;
+          uint16_t *to = a.vn + part * a.vn_part + panel_at(end_v, row, col);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float e[4] = {acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
+            uint2 x;
+            x.x = take(e[0]);
+            x.x |= take(e[1]) << 16;
+            x.y = take(e[2]);
+            x.y |= take(e[3]) << 16;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc.c[i][j][4 * q + k] = e[k];
+            const uint2 y = turn4(x, lane);
+            if (kInside || (row + 8 * q < end_v && col < end_n)) *reinterpret_cast<uint2 *>(to + 8 * q * kStepK) = y;
+          }
+        }
+      }
+    };
+#pragma unroll
+    for (int part = 0; part < Multiply<T>::kParts; ++part) {
+      if (sizeof(T) == 2 && whole) store(std::true_type{}, part);  // a second copy of the code costs float32 its registers
+      else store(std::false_type{}, part);
+    }
+    clear(acc);
+  });
 }
 
 struct StoreArgs {
@@ -658,11 +674,11 @@ double rounds_time(const TileSize &s, int64_t groups, double work) {
 // Ranges of the vocabulary tiles for the statistics: the division with the shortest time, each workgroup costing about
 // three microseconds to begin.
 constexpr int kMostRanges = 256;
-double choose_ranges(const TileSize &s, int64_t M, int64_t N, int64_t steps, int *ranges) {
+double choose_ranges(const TileSize &s, int64_t M, int64_t N, int64_t steps, double epilogue, int *ranges) {
   const int64_t tiles_m = tiles_of(M, s.bm), tiles_n = tiles_of(N, s.bn);
   double least = 0.0;
   for (int64_t r = 1; r <= std::min<int64_t>(tiles_m, kMostRanges); ++r) {
-    const double t = rounds_time(s, tiles_n * r, static_cast<double>(tiles_of(tiles_m, r)) * (steps * s.step + s.stats) + 3.0);
+    const double t = rounds_time(s, tiles_n * r, static_cast<double>(tiles_of(tiles_m, r)) * (steps * s.step + epilogue) + 3.0);
     if (r == 1 || t < least) {
       *ranges = static_cast<int>(r);
       least = t;
@@ -747,12 +763,11 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   const int64_t steps = steps_of(D) * l.segments;
   if (!backward) {
     int ranges;
-    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, &ranges); });
+    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, s.stats, &ranges); });
     l.stats = take(l.pieces * std::min<int64_t>(tiles_of(l.piece, kTileSize[l.logits].bm), kMostRanges) * N * 8);
   } else {
-    l.logits = choose_tile([&](const TileSize &s) {
-      return rounds_time(s, tiles_of(in_piece, s.bm) * tiles_of(N, s.bn), steps * s.step + l.parts * s.grad);
-    });
+    int ranges;
+    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, l.parts * s.grad, &ranges); });
     int z;
     const int64_t dh_steps = steps_of(in_piece) * l.segments, dw_steps = steps_of(N) * l.segments;
     l.dh = choose_tile([&](const TileSize &s) { return choose_splits(s, N, D, dh_steps, &z); });
@@ -859,7 +874,7 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
     a.v0 = v0;
     const int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3) {
       using Tile = decltype(tile);
-      choose_ranges(kTileSize[l.logits], a.g.a.rows, N, steps_of(D) * l.segments, &a.ranges);
+      choose_ranges(kTileSize[l.logits], a.g.a.rows, N, steps_of(D) * l.segments, kTileSize[l.logits].stats, &a.ranges);
       stats_kernel<Tile, T, Id><<<dim3(static_cast<unsigned>(a.ranges * a.g.tiles_n)), dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
@@ -921,9 +936,11 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     if (l.packed) copy_rows<T>(rows_of, stream);
     copy_transposed<T>(transposed, stream);
     rows_of.job[0].rows = transposed.job[0].rows = 0;  // h is there now
-    int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3 grid) {
+    int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3) {
       using Tile = decltype(tile);
-      grad_logits_kernel<Tile, T><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
+      const TileSize &size = kTileSize[l.logits];
+      choose_ranges(size, rows, N, steps_of(D) * l.segments, l.parts * size.grad, &a.ranges);
+      grad_logits_kernel<Tile, T><<<dim3(static_cast<unsigned>(a.ranges * a.g.tiles_n)), dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
 
