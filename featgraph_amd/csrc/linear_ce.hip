@@ -653,10 +653,10 @@ struct TileSize {
   double stats, grad, store;        // ... per tile for the epilogues of the three kernels (16-bit results)
 };
 // Measured on products of 1024 .. 8192 terms and epilogues of 4096 x 65536 logits.
-constexpr TileSize kTileSize[] = {{256, 256, 1, 1.95, 3.0, 15.0, 6.0},
-                                  {128, 128, 2, 1.15, 1.8, 9.0, 3.5},
-                                  {64, 256, 2, 1.25, 1.8, 9.0, 3.5},
-                                  {256, 64, 2, 1.25, 1.8, 9.0, 3.5}};
+constexpr TileSize kTileSize[] = {{256, 256, 1, 1.95, 3.1, 12.0, 6.0},
+                                  {128, 128, 2, 1.15, 1.4, 5.7, 3.5},
+                                  {64, 256, 2, 1.25, 1.4, 6.0, 3.5},
+                                  {256, 64, 2, 1.25, 1.4, 6.0, 3.5}};
 constexpr int kCus = 256;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
