@@ -447,6 +447,7 @@ int *config_slot(const char *key) {
   fg::Config &c = fg::config();
   if (!key) return nullptr;
   if (!strcmp(key, "ce.tile")) return &c.ce_tile;
+  if (!strcmp(key, "ce.native")) return &c.ce_native;
   if (!strcmp(key, "ce.piece_rows")) return &c.ce_piece_rows;
   if (!strcmp(key, "spmm.vec")) return &c.spmm_vec;
   if (!strcmp(key, "spmm.lpr")) return &c.spmm_lpr;
@@ -1133,7 +1134,8 @@ int fg_config_set(const char *key, int32_t value) {
                     slot == &fg::config().spmm_multi || slot == &fg::config().sddmm_sorted_copy ||
                     slot == &fg::config().sddmm_regroup || slot == &fg::config().spmm_relay ||
                     slot == &fg::config().spmm_general_multi || slot == &fg::config().sddmm_xcd ||
-                    slot == &fg::config().spmm_xcd || slot == &fg::config().spmm_pad_rows;
+                    slot == &fg::config().spmm_xcd || slot == &fg::config().spmm_pad_rows ||
+                    slot == &fg::config().ce_native;
   // flags: 0 / 1 are explicit, anything negative restores the default;
   // sizes: 0 restores the default
   *slot = flag ? (value < 0 ? -1 : (value != 0)) : std::max(value, 0);

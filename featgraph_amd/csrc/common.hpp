@@ -31,7 +31,7 @@ struct Config {
   int attention_blocks = 0, sddmm_rows_wide = 0, sddmm_sorted_copy = -1, sddmm_regroup = -1, spmm_relay = -1, spmm_general_multi = -1;
   int sddmm_xcd = -1, spmm_xcd = -1;
   int spmm_pad_rows = -1;
-  int ce_tile = 0, ce_piece_rows = 0;
+  int ce_tile = 0, ce_piece_rows = 0, ce_native = -1;
 };
 Config &config();
 

@@ -14,7 +14,8 @@
 //
 // Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step of each
 // term, random in sign; the results are rounded to bfloat16 themselves); everything between is float32.  float32
-// operands, P among them, are split into two float16 parts (mfma_gemm.hpp), which keeps float32's accuracy.  P is at
+// operands, P among them, are split into two float16 parts (mfma_gemm.hpp), which keeps float32's accuracy; the loss
+// multiplies them as they are where reading one of them bounds it (few rows, or few classes).  P is at
 // most 1 and stored times 2^14; dloss is applied to the rows of dh in the epilogue and to the copy of h for dw.
 #include <algorithm>
 #include <cmath>
@@ -278,7 +279,7 @@ __device__ __forceinline__ GemmPlace range_place(const GemmShape &g, int ranges,
 
 // A workgroup takes one tile of rows n and a range of the vocabulary, tile after tile without a pause in its loads; each
 // lane keeps the statistics of the logits it meets (its column n, half the rows of its wave) until the end.
-template <typename Tile, typename T, typename Id>
+template <typename Tile, typename T, typename M, typename Id>
 __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint16_t lds[Tile::kLds];
   GemmAcc<Tile> acc;
@@ -297,9 +298,9 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
     sum[j] = 0.0f;
     label[j] = n < a.g.b.rows ? static_cast<int64_t>(static_cast<const Id *>(a.labels)[n]) - a.v0 - first_v : -1;
   }
-  gemm_tiles<Tile, T, false>(a.g, at, tiles, lds, acc, [&](int tile) {
+  gemm_tiles<Tile, M, false>(a.g, at, tiles, lds, acc, [&](int tile) {
     const int64_t v0 = first_v + static_cast<int64_t>(tile) * Tile::BM;
-    to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
+    if constexpr (M::kSegments > 1) to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
 #pragma unroll
     for (int j = 0; j < Tile::TN; ++j) {
       if (v0 + Tile::BM / Tile::WM > a.g.a.rows) {
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
     }
     return bits;
   };
-  gemm_tiles<Tile, T, false>(a.g, at, tiles, lds, acc, [&](int tile) {
+  gemm_tiles<Tile, Multiply<T>, false>(a.g, at, tiles, lds, acc, [&](int tile) {
     const int v0 = first_v + tile * Tile::BM;
     to_logits<Tile, T>(acc, a.exp_a, a.exp_b, v0, n0, a.g.b.rows, lane);
 #pragma unroll
@@ -657,6 +658,12 @@ constexpr TileSize kTileSize[] = {{256, 256, 1, 1.95, 3.1, 12.0, 6.0},
                                   {128, 128, 2, 1.15, 1.4, 5.7, 3.5},
                                   {64, 256, 2, 1.25, 1.4, 6.0, 3.5},
                                   {256, 64, 2, 1.25, 1.4, 6.0, 3.5}};
+// Native float32: the step is 32 k, bound by the float32 matrix instructions.
+constexpr TileSize kNativeSize[] = {{256, 256, 1, 7.8, 3.1, 0.0, 0.0},
+                                    {128, 128, 2, 3.9, 1.4, 0.0, 0.0},
+                                    {64, 256, 2, 3.9, 1.4, 0.0, 0.0},
+                                    {256, 64, 2, 3.9, 1.4, 0.0, 0.0}};
+constexpr double kBytesPerUs = 4.5e6;  // that a pass over memory reaches
 constexpr int kCus = 256;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
@@ -676,13 +683,16 @@ double rounds_time(const TileSize &s, int64_t groups, double work) {
 constexpr int kMostRanges = 256;
 double choose_ranges(const TileSize &s, int64_t M, int64_t N, int64_t steps, double epilogue, int *ranges) {
   const int64_t tiles_m = tiles_of(M, s.bm), tiles_n = tiles_of(N, s.bn);
-  double least = 0.0;
-  for (int64_t r = 1; r <= std::min<int64_t>(tiles_m, kMostRanges); ++r) {
-    const double t = rounds_time(s, tiles_n * r, static_cast<double>(tiles_of(tiles_m, r)) * (steps * s.step + epilogue) + 3.0);
-    if (r == 1 || t < least) {
+  double least = -1.0;
+  for (int64_t each = tiles_of(tiles_m, kMostRanges); each <= tiles_m;) {  // tiles per workgroup
+    const int64_t r = tiles_of(tiles_m, each);
+    const double t = rounds_time(s, tiles_n * r, static_cast<double>(each) * (steps * s.step + epilogue) + 3.0);
+    if (least < 0.0 || t < least) {
       *ranges = static_cast<int>(r);
       least = t;
     }
+    if (r == 1) break;
+    each = tiles_of(tiles_m, r - 1);  // the next one that needs fewer ranges
   }
   return least;
 }
@@ -703,19 +713,21 @@ double choose_splits(const TileSize &s, int64_t M, int64_t N, int64_t steps, int
   return least;
 }
 
-// The kind of tile with the shortest time by `cost`.
+// The kind of tile with the shortest time by `cost`, which goes to *time.
 template <typename F>
-TileKind choose_tile(F &&cost) {
-  if (const int forced = config().ce_tile) return static_cast<TileKind>(std::min(forced, 4) - 1);
+TileKind choose_tile(F &&cost, const TileSize *sizes = kTileSize, double *time = nullptr) {
   int best = kBig;
   double least = 0.0;
+  const int forced = config().ce_tile;
   for (int k = 0; k < 4; ++k) {
-    const double t = cost(kTileSize[k]);
-    if (k == 0 || t < least) {
+    if (forced && k != std::min(forced, 4) - 1) continue;
+    const double t = cost(sizes[k]);
+    if (forced || k == 0 || t < least) {
       best = k;
       least = t;
     }
   }
+  if (time) *time = least;
   return static_cast<TileKind>(best);
 }
 
@@ -727,6 +739,8 @@ constexpr int64_t kPieceBytes = int64_t{4} << 30;
 struct Layout {
   int parts, segments;
   int64_t pieces;
+  int ranges;            // of a piece's vocabulary tiles
+  bool native;           // float32 multiplied as it is (loss only)
   bool packed;           // operands copied with k padded (float32, or rows that are no multiple of kStepK or 16 bytes)
   int64_t piece;         // vocabulary rows per piece, a multiple of 256
   TileKind logits, dh, dw;
@@ -738,7 +752,18 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   Layout l{};
   l.parts = dtype == FG_F32 ? kParts : 1;
   l.segments = dtype == FG_F32 ? kSegments : 1;
-  l.packed = dtype == FG_F32 || D % kStepK != 0 || !aligned;
+  if (dtype == FG_F32 && !backward) {
+    // as they are, against three products of copies, which are written once and read twice (with a launch of their own)
+    double split, native;
+    int r;
+    choose_tile([&](const TileSize &s) { return choose_ranges(s, V, N, steps_of(D) * kSegments, s.stats, &r); }, kTileSize, &split);
+    choose_tile([&](const TileSize &s) { return choose_ranges(s, V, N, steps_of(2 * D), s.stats, &r); }, kNativeSize, &native);
+    const double bytes = 4.0 * static_cast<double>(N + V) * static_cast<double>(D);
+    l.native = std::max(native, bytes / kBytesPerUs) < split + 5.0 + 3.0 * bytes / kBytesPerUs;
+    if (config().ce_native >= 0) l.native = config().ce_native != 0;
+  }
+  if (l.native) l.segments = 1;
+  l.packed = !l.native && (dtype == FG_F32 || D % kStepK != 0 || !aligned);
   int64_t per_row = l.packed ? 2 * l.parts * up(D, kStepK) : 0;
   if (backward) per_row += 2 * l.parts * (up(N, kStepK) + D);
   // at most 2^22 rows, which 32-bit offsets into four panels reach
@@ -755,19 +780,20 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   };
   l.h_pack = take(l.packed ? 2 * l.parts * panel_elements(N, D) : 0);
   l.w_pack = take(l.packed ? 2 * l.parts * panel_elements(in_piece, D) : 0);
-  if (dtype == FG_F32) {
+  if (l.packed && dtype == FG_F32) {
     l.h_exp = take(4 * up(N, 256));
     l.w_exp = take(4 * up(in_piece, 256));
     l.peaks = take(4 * kPeakSlots * kPeakStride * (1 + l.pieces));
   }
-  const int64_t steps = steps_of(D) * l.segments;
+  const int64_t steps = l.native ? steps_of(2 * D) : steps_of(D) * l.segments;
   if (!backward) {
-    int ranges;
-    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, s.stats, &ranges); });
+    const TileSize *sizes = l.native ? kNativeSize : kTileSize;
+    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, s.stats, &l.ranges); }, sizes);
+    choose_ranges(sizes[l.logits], in_piece, N, steps, sizes[l.logits].stats, &l.ranges);
     l.stats = take(l.pieces * std::min<int64_t>(tiles_of(l.piece, kTileSize[l.logits].bm), kMostRanges) * N * 8);
   } else {
-    int ranges;
-    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, l.parts * s.grad, &ranges); });
+    l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, l.parts * s.grad, &l.ranges); });
+    choose_ranges(kTileSize[l.logits], in_piece, N, steps, l.parts * kTileSize[l.logits].grad, &l.ranges);
     int z;
     const int64_t dh_steps = steps_of(in_piece) * l.segments, dw_steps = steps_of(N) * l.segments;
     l.dh = choose_tile([&](const TileSize &s) { return choose_splits(s, N, D, dh_steps, &z); });
@@ -814,7 +840,7 @@ GemmOperand operand(const CopyJob &job, const Layout &l) {
   GemmOperand o;
   o.rows = static_cast<int32_t>(job.rows);
   o.p = static_cast<const uint16_t *>(job.x);
-  o.row = job.D;
+  o.row = job.D * static_cast<int64_t>(sizeof(T) / 2);
   o.step = kStepK;
   return o;
 }
@@ -859,7 +885,8 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
   a.labels = labels;
   a.label_logit = loss;
   a.part = reinterpret_cast<float2 *>(ws + l.stats);
-  a.g.steps = static_cast<int32_t>(steps_of(D));
+  a.g.steps = static_cast<int32_t>(steps_of(l.native ? 2 * D : D));
+  a.g.tail = static_cast<int32_t>(l.native ? 2 * D - (a.g.steps - 1) * kStepK : kStepK);
   auto *h_exp = reinterpret_cast<int32_t *>(ws + l.h_exp), *w_exp = reinterpret_cast<int32_t *>(ws + l.w_exp);
   a.exp_a = w_exp;
   a.exp_b = h_exp;
@@ -874,8 +901,15 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
     a.v0 = v0;
     const int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3) {
       using Tile = decltype(tile);
-      choose_ranges(kTileSize[l.logits], a.g.a.rows, N, steps_of(D) * l.segments, kTileSize[l.logits].stats, &a.ranges);
-      stats_kernel<Tile, T, Id><<<dim3(static_cast<unsigned>(a.ranges * a.g.tiles_n)), dim3(Tile::kThreads), 0, stream>>>(a);
+      a.ranges = std::min(l.ranges, a.g.tiles_m);
+      const dim3 grid(static_cast<unsigned>(a.ranges * a.g.tiles_n));
+      if constexpr (sizeof(T) == 4) {
+        if (l.native) {
+          stats_kernel<Tile, T, MultiplyNative, Id><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
+          return;
+        }
+      }
+      stats_kernel<Tile, T, Multiply<T>, Id><<<grid, dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;
     a.range0 += a.ranges;
@@ -938,8 +972,7 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     rows_of.job[0].rows = transposed.job[0].rows = 0;  // h is there now
     int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3) {
       using Tile = decltype(tile);
-      const TileSize &size = kTileSize[l.logits];
-      choose_ranges(size, rows, N, steps_of(D) * l.segments, l.parts * size.grad, &a.ranges);
+      a.ranges = std::min(l.ranges, a.g.tiles_m);
       grad_logits_kernel<Tile, T><<<dim3(static_cast<unsigned>(a.ranges * a.g.tiles_n)), dim3(Tile::kThreads), 0, stream>>>(a);
     });
     if (rc) return rc;

@@ -63,6 +63,22 @@ struct Multiply<float> {
   }
 };
 
+// float32 operands as they are, on the float32 matrix instructions: a fragment of 16 bytes is four k.  A sixth of the
+// rate, but no copies: for products that are bound by reading one of the operands.
+struct MultiplyNative {
+  static constexpr int kParts = 1, kSegments = 1;
+  static __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[k], y[k], c, 0, 0, 0);
+#endif
+    return c;
+  }
+};
+
+// Elements are 16 bits; a native float32 counts as two.
 struct GemmOperand {
   const uint16_t *p = nullptr;  // part 0
   int64_t part = 0;             // elements from one part to the next
@@ -100,6 +116,7 @@ struct GemmShape {
   GemmOperand a, b;
   int32_t steps = 0;   // of kStepK per part
   int32_t splits = 1;  // workgroups that share one tile's k range
+  int32_t tail = kStepK;  // native: elements of the last step that exist (the others are whole in copies and in place)
   int32_t tiles_m = 0, tiles_n = 0;
 };
 
@@ -173,12 +190,12 @@ __device__ __forceinline__ void clear(GemmAcc<Tile> &acc) {
       for (int r = 0; r < 16; ++r) acc.c[i][j][r] = 0.0f;
 }
 
-template <typename Tile, typename T, bool kTurnA, typename Done>
+template <typename Tile, typename M, bool kTurnA, typename Done>
 __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &at, int tiles, uint16_t *lds,
                                            GemmAcc<Tile> &acc, Done &&done) {
 #if defined(__HIP_DEVICE_COMPILE__)  // the host pass lacks the loads to LDS
   using LdsPtr = __attribute__((address_space(3))) void *;
-  using M = Multiply<T>;
+  constexpr bool kNative = std::is_same<M, MultiplyNative>::value;
   constexpr int kLoads = Tile::kLoadsA + Tile::kLoadsB;
   const int lane = threadIdx.x & (kWaveSize - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
@@ -226,8 +243,8 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     if constexpr (decltype(turned)::value)
       c.bytes = ((there + kStepK - 1) / kStepK - 1) * (static_cast<uint32_t>(o.row) * (kStepK * 2)) + kStepK * kStepK * 2;
     else
-      c.bytes = (there - 1) * static_cast<uint32_t>(o.row * 2) + kStepK * 2;
-    c.until = min(g.steps - step, c.tile_left);
+      c.bytes = (there - 1) * static_cast<uint32_t>(o.row * 2) + (kNative && step == g.steps - 1 ? g.tail : kStepK) * 2;
+    c.until = min(kNative && step < g.steps - 1 ? g.steps - 1 - step : g.steps - step, c.tile_left);
   };
   auto advance = [&](Cursor &c, const GemmOperand &o, int64_t &row, int rows, int stride, int hi_segment, int stages, auto turned) {
     if (++c.slot == stages) c.slot = 0;
@@ -236,8 +253,8 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     if (--c.left <= 0) {
       c.bytes = 0;
     } else if (--c.until == 0) {
-      int step = 0;
-      ++c.seg;
+      int step = kNative ? g.steps - 1 : 0;  // native: the last step, whose rows may end early
+      if (!kNative) ++c.seg;
       if (c.tile_left == 0) {
         c.tile_left = per_tile;
         c.seg = first_seg;
@@ -290,6 +307,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     Rows lines[kTurnA ? 8 : 1];
   };
   int slot_a = 0, slot_b = 0;  // of the step that is read
+  int left_in_tile = per_tile;  // steps from it to the tile's end
   auto read = [&](Fragments &f, int quarter) {
     const int piece = ((2 * quarter + lane / 32) ^ twist) * 8;
     const uint16_t *sb = lds_b + slot_b * Tile::kStageB + at_b + piece;
@@ -304,6 +322,22 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     }
 #pragma unroll
     for (int t = 0; t < Tile::TN; ++t) f.b[t] = *reinterpret_cast<const bf16x8 *>(sb + t * 32 * kStepK);
+    if constexpr (kNative) {
+      if (left_in_tile == 1 && g.tail < kStepK) {  // what lies behind the rows' ends belongs to the next rows
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const int first_k = (2 * quarter + lane / 32) * 4, end_k = g.tail / 2;
+        auto cut = [&](bf16x8 &x) {
+          u32x4 w = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = first_k + k < end_k ? w[k] : 0;
+          x = __builtin_bit_cast(bf16x8, w);
+        };
+#pragma unroll
+        for (int t = 0; t < Tile::TM; ++t) cut(f.a[t]);
+#pragma unroll
+        for (int t = 0; t < Tile::TN; ++t) cut(f.b[t]);
+      }
+    }
   };
   // kQuarter of the period, whose share of the loads goes out between the products
   auto multiply = [&](const Fragments &f, auto quarter) {
@@ -376,6 +410,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
     arrive_and_meet<kDeep ? Tile::kLoadsA : 0>();
     if (++slot_a == Tile::kStagesA) slot_a = 0;
     slot_b ^= 1;
+    if (--left_in_tile == 0) left_in_tile = per_tile;
     read(f0, 0);  // past the last step: what is read is not used
     multiply(f1, Q0{});
     if (++in_tile == per_tile) {
@@ -392,7 +427,7 @@ __device__ __forceinline__ void gemm_tiles(const GemmShape &g, const GemmPlace &
 // One tile, left in acc.
 template <typename Tile, typename T, bool kTurnA = false>
 __device__ __forceinline__ void gemm_tile(const GemmShape &g, const GemmPlace &at, uint16_t *lds, GemmAcc<Tile> &acc) {
-  gemm_tiles<Tile, T, kTurnA>(g, at, 1, lds, acc, [](int) {});
+  gemm_tiles<Tile, Multiply<T>, kTurnA>(g, at, 1, lds, acc, [](int) {});
 }
 
 }  // namespace fg

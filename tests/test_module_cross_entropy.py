@@ -104,6 +104,7 @@ def config():
     yield _lib.config_set
     _lib.config_set("ce.tile", 0)
     _lib.config_set("ce.piece_rows", 0)
+    _lib.config_set("ce.native", -1)
 
 
 @pytest.mark.gpu
@@ -117,6 +118,26 @@ def test_every_tile_and_pieces_of_the_vocabulary(config, dtype, tile, N, V, D, p
     first = _run(h, w, y, dl, dtype)
     _reference(h, w, y, dl, dtype, *first)
     assert all(torch.equal(a, b) for a, b in zip(first, _run(h, w, y, dl, dtype)))      # the same bits again
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [0, 1])
+@pytest.mark.parametrize("tile", [1, 2, 3, 4])
+@pytest.mark.parametrize("N,V,D", [(70, 600, 1), (33, 300, 30), (257, 100, 33), (40, 1500, 64), (300, 41, 127), (5, 2000, 447)])
+def test_float32_as_copies_and_as_it_is(config, native, tile, N, V, D):
+    """Rows of every length modulo 16 bytes and 32 elements; rows of NaN between the others reach nothing but themselves."""
+    config("ce.native", native)
+    config("ce.tile", tile)
+    h, w, y, dl = _operands("float32", N, V, D, tile + D, ignored=0.3)
+    ph = [placeholder((N, D)), placeholder((V, D)), placeholder((N,), "int32")]
+    f = LinearCrossEntropyhip()
+    f.build(ph)
+    loss, lse = (x.tensor.clone() for x in f.run([h, w, y]))
+    _reference(h, w, y, dl, "float32", loss, lse, None, None)
+    bad = (y < 0) | (y >= V)
+    h[bad] = float("nan")
+    loss2, lse2 = f.run([h, w, y])
+    assert torch.equal(loss2.tensor, loss) and torch.equal(lse2.tensor[~bad], lse[~bad])
 
 
 @pytest.mark.gpu
