@@ -90,7 +90,7 @@ def _run(h, w, y, dl, dtype, itype="int32"):
 @pytest.mark.parametrize("dtype", list(TYPES))
 @pytest.mark.parametrize("N,V,D", [(1, 1, 1), (5, 3, 2), (64, 41, 64), (127, 255, 100), (33, 300, 64), (300, 70, 130),
                                    (257, 1025, 192), (70, 5000, 72), (1000, 41, 256), (20, 30001, 40), (1, 4096, 64),
-                                   (2049, 513, 24), (9, 1, 5)])
+                                   (2049, 513, 24), (9, 1, 5), (20, 50, 600), (17, 40, 1100)])
 def test_loss_and_gradients(dtype, N, V, D):
     itype = "int64" if N % 2 else "int32"
     h, w, y, dl = _operands(dtype, N, V, D, N + V + D, itype=itype)
