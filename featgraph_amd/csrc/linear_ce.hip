@@ -761,6 +761,7 @@ TileKind choose_tile(F &&cost, const TileSize *sizes = kTileSize, double *time =
 // would hold, cost more in short launches than the cache gives back (4096 x 65536 x 1024: 2371 us for the gradient in
 // pieces of 256 MiB, 2005 of 512, 1891 of 1024, 1780 in one).
 constexpr int64_t kPieceBytes = int64_t{4} << 30;
+constexpr int64_t kMostPieceRows = 1 << 22;  // which 32-bit offsets into four panels reach
 
 struct Layout {
   int parts, segments;
@@ -792,10 +793,9 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
   l.packed = !l.native && (dtype == FG_F32 || D % kStepK != 0 || !aligned);
   int64_t per_row = l.packed ? 2 * l.parts * up(D, kStepK) : 0;
   if (backward) per_row += 2 * l.parts * (up(N, kStepK) + D);
-  // at most 2^22 rows, which 32-bit offsets into four panels reach
-  const int64_t most = per_row ? std::clamp<int64_t>(kPieceBytes / per_row / 256 * 256, 256, 1 << 22) : up(V, 256);
+  const int64_t most = per_row ? std::clamp<int64_t>(kPieceBytes / per_row / 256 * 256, 256, kMostPieceRows) : up(V, 256);
   l.piece = up((V + (V + most - 1) / most - 1) / ((V + most - 1) / most), 256);  // as many pieces as needed, of equal size
-  if (const int64_t rows = config().ce_piece_rows) l.piece = up(rows, 256);
+  if (const int64_t rows = config().ce_piece_rows) l.piece = std::min(up(rows, 256), kMostPieceRows);
   const int64_t in_piece = std::min(l.piece, V);
   l.pieces = (V + l.piece - 1) / l.piece;
   int64_t at = 0;

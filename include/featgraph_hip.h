@@ -512,7 +512,8 @@ FG_API int64_t fg_probe_gather_stream_f32(const float *feat, int32_t band_rows, 
  * vertex row per wave when a row is 1 KB or more, else 65536 workgroups that
  * walk the rows), "ce.tile" (1..4: the 256 x 256, 128 x 128, 64 x 256 or 256 x 64
  * tile for every product of fg_linear_ce and fg_linear_ce_grad), "ce.piece_rows"
- * (vocabulary rows per piece of those calls, rounded up to a multiple of 256),
+ * (vocabulary rows per piece of those calls, rounded up to a multiple of 256,
+ * at most 4194304),
  * "ce.native" (0/1: whether fg_linear_ce multiplies float32 operands as copies
  * in float16 parts or as they are; by default what is faster for the sizes);
  * all are read by the calls and by the functions that size their workspaces.

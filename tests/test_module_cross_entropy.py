@@ -326,3 +326,19 @@ def test_bad_arguments_of_the_entry_points_without_a_device():
     assert L.fg_linear_ce_grad_workspace(4, 4, 4, 0, ctypes.byref(need)) == 0
     assert L.fg_linear_ce_grad(4, 4, 4, 16, 16, 16, 16, None, 16, 16, 0, 0, 256, need.value, None) == -1
     assert L.fg_linear_ce_grad(4, 4, 4, 16, 16, 16, 16, 16, 16, 16, 0, 0, 264, need.value, None) == -1
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_pieces_stay_within_32_bit_offsets(dtype):
+    """The kernels reach 2^22 vocabulary rows of a piece with 32-bit offsets: a larger wish gives pieces of that size."""
+    L = _lib.lib()
+    sizes = []
+    try:
+        for rows in (2 ** 22, 2 ** 22 + 1, 2 ** 30, 2 ** 31 - 1):
+            _lib.config_set("ce.piece_rows", rows)
+            need = ctypes.c_int64(0)
+            assert L.fg_linear_ce_grad_workspace(64, 2 ** 24, 64, dtype, ctypes.byref(need)) == 0
+            sizes.append(need.value)
+    finally:
+        _lib.config_set("ce.piece_rows", 0)
+    assert len(set(sizes)) == 1, sizes
