@@ -88,7 +88,8 @@ class ClipGradNormhip(GradNormhip):
         if not self._in_place:
             self._clipped = [NDArray(torch.zeros(shape, dtype=t, device=self._ctx)) for shape, t, _ in self._expected]
             self._out[:] = [c.tensor.data_ptr() for c in self._clipped]
-            spans = sorted((c.tensor.data_ptr(), size) for c, (_, _, size) in zip(self._clipped, self._expected) if size)
+            spans = sorted([(c.tensor.data_ptr(), size) for c, (_, _, size) in zip(self._clipped, self._expected) if size] +
+                           [(self._norm.tensor.data_ptr(), 4)])
             self._out_begin, self._out_end = [b for b, _ in spans], [b + n for b, n in spans]
         self._built = True
 
@@ -96,9 +97,10 @@ class ClipGradNormhip(GradNormhip):
         tensors, at = super()._checked(arrays)
         if self._in_place:
             end = 0
-            for begin, size in sorted((b, size) for b, (_, _, size) in zip(at, self._expected) if size):
+            for begin, size in sorted([(b, size) for b, (_, _, size) in zip(at, self._expected) if size] +
+                                      [(self._norm.tensor.data_ptr(), 4)]):
                 if begin < end:
-                    raise ValueError("the gradients overlap each other")
+                    raise ValueError("the gradients overlap each other or the module's norm")
                 end = begin + size
         else:
             begins, ends = self._out_begin, self._out_end

@@ -186,6 +186,18 @@ def test_refusals():
     two.run([x[:24].repeat(2)[:40], x[:40]])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+def test_the_norm_is_no_gradient_of_the_same_call(in_place):
+    m = ClipGradNormhip(1.0)
+    m.build([placeholder((1,)), placeholder((8,))], {"in_place": in_place})
+    x = torch.ones(8, device="cuda")
+    norm, _ = m.run([torch.ones(1, device="cuda"), x])
+    assert float(norm.tensor) == 3.0
+    with pytest.raises(ValueError):
+        m.run([norm.tensor.reshape(1), x])
+
+
 def test_bad_arguments_of_the_entry_points_without_a_device():
     L = _lib.lib()
     need = ctypes.c_int64(0)
