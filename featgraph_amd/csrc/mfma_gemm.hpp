@@ -9,7 +9,8 @@
 // accuracy at a third of the 16-bit rate, 5.3 times the peak rate of the float32 matrix instructions.
 //
 // A workgroup computes a BM x BN tile in steps of 64 k.  The operands' rows go straight to LDS (16 bytes per lane, whole
-// 128-byte lines, no registers in between) into one of two stages.  The fragments of each quarter of a step are read
+// 128-byte lines, no registers in between) into the next of two stages of B and, where LDS allows, three of A: then only
+// the loads of the step's second half have to arrive within it.  The fragments of each quarter of a step are read
 // while the quarter before it multiplies, over the border of the steps too: the waves meet before the last quarter, when
 // its fragments are in registers, the next stage has arrived and this one can be filled again.  A tile row is 128 bytes
 // in LDS; its eight 16-byte pieces are placed at (piece ^ (row / 2 % 8)), so that the lanes of a fragment read, which

@@ -554,6 +554,7 @@ FG_API int fg_sddmm_describe(int64_t nnz, int32_t H, int32_t D, char *buf, int64
 /*
  * out[i, :] = scale * table[ids[i], :] for table [n_rows, D] and out
  * [n_ids, D].  An id outside [0, n_rows) is padding: its row becomes zero.
+ * out must not overlap table or ids.
  */
 FG_API int fg_embedding_lookup(int64_t n_rows, int64_t D, int64_t n_ids, const void *table, const void *ids, void *out,
                                float scale, int32_t dtype, int32_t itype, void *stream);
@@ -619,7 +620,9 @@ FG_API int fg_linear_ce(int64_t N, int64_t V, int64_t D, const void *hidden, con
  * dweight, whatever their hidden row, lse and dloss hold.  The logits are
  * computed again, a piece of the vocabulary at a time.  With bfloat16 operands
  * G is rounded to bfloat16; with float32 everything keeps float32's accuracy.
- * dhidden and dweight must not overlap each other or an input.
+ * dhidden and dweight must not overlap each other or an input.  lse has to be
+ * the forward call's for the same operands: far smaller values take G beyond
+ * the range it is kept in.
  */
 FG_API int fg_linear_ce_grad_workspace(int64_t N, int64_t V, int64_t D, int32_t dtype, int64_t *bytes);
 FG_API int fg_linear_ce_grad(int64_t N, int64_t V, int64_t D, const void *hidden, const void *weight, const void *labels,
