@@ -430,6 +430,25 @@ __device__ __forceinline__ uint2 turn4(uint2 x, int lane) {
 #endif
 }
 
+// After turn4 of the two blocks of a wave's 64 columns: neighbouring fours of lanes exchange halves, so that a lane holds
+// eight neighbouring columns of its row and eight lanes a whole line, at columns line_column() on.  Stores of half lines
+// reached 2 TB/s where whole lines reach STORERATE.
+__device__ __forceinline__ uint4 line_of(uint2 first, uint2 second, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  auto swap4 = [](uint32_t x) {  // lane ^ 4: fours 0 and 2 of a row take from above, 1 and 3 from below
+    constexpr int kUp4 = 0x104, kDown4 = 0x114;  // from lane + 4, from lane - 4
+    const int up = __builtin_amdgcn_update_dpp(0, static_cast<int>(x), kUp4, 0xf, 0x5, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(up, static_cast<int>(x), kDown4, 0xf, 0xa, false));
+  };
+  const bool odd = lane & 4;
+  const uint32_t x = swap4(odd ? first.x : second.x), y = swap4(odd ? first.y : second.y);
+  return odd ? uint4{x, y, second.x, second.y} : uint4{first.x, first.y, x, y};
+#else
+  return uint4{first.x, first.y, second.x, second.y};
+#endif
+}
+__device__ __forceinline__ int line_column(int lane) { return lane / 4 % 2 * 32 + lane % 32 / 8 * 8; }
+
 struct GradArgs {
   GemmShape g;               // a: the piece's rows of w, b: h
   const int32_t *exp_a, *exp_b;
@@ -509,27 +528,29 @@ __global__ __launch_bounds__(Tile::kThreads) void grad_logits_kernel(GradArgs a)
     const bool whole = v0 + Tile::BM / Tile::WM <= M && n0 + Tile::BN / Tile::WN <= N;
     auto store = [&](auto inside, int part) {  // inside: the wave's whole block lies within the matrix
       constexpr bool kInside = decltype(inside)::value;
+      static_assert(Tile::TN == 2, "a wave's columns are a line");
+      const int64_t col = n0 + line_column(lane);
 #pragma unroll
-      for (int j = 0; j < Tile::TN; ++j) {
-        const int64_t col = n0 + 32 * j + lane % 32 / 4 * 4;
+      for (int i = 0; i < Tile::TM; ++i) {
+        FG_IN_ORDER();
+        const int64_t row = v0 + 32 * i + acc_row(0, lane) + lane % 4;
+        uint16_t *to = a.vn + part * a.vn_part + panel_at(end_v, row, col);
 #pragma unroll
-        for (int i = 0; i < Tile::TM; ++i) {
-          FG_IN_ORDER();
-          const int64_t row = v0 + 32 * i + acc_row(0, lane) + lane % 4;
-          uint16_t *to = a.vn + part * a.vn_part + panel_at(end_v, row, col);
+        for (int q = 0; q < 4; ++q) {
+          uint2 x[2];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int j = 0; j < 2; ++j) {
             float e[4] = {acc.c[i][j][4 * q], acc.c[i][j][4 * q + 1], acc.c[i][j][4 * q + 2], acc.c[i][j][4 * q + 3]};
-            uint2 x;
-            x.x = take(e[0]);
-            x.x |= take(e[1]) << 16;
-            x.y = take(e[2]);
-            x.y |= take(e[3]) << 16;
+            x[j].x = take(e[0]);
+            x[j].x |= take(e[1]) << 16;
+            x[j].y = take(e[2]);
+            x[j].y |= take(e[3]) << 16;
 #pragma unroll
             for (int k = 0; k < 4; ++k) acc.c[i][j][4 * q + k] = e[k];
-            const uint2 y = turn4(x, lane);
-            if (kInside || (row + 8 * q < end_v && col < end_n)) *reinterpret_cast<uint2 *>(to + 8 * q * kStepK) = y;
+            x[j] = turn4(x[j], lane);
           }
+          const uint4 y = line_of(x[0], x[1], lane);
+          if (kInside || (row + 8 * q < end_v && col < end_n)) *reinterpret_cast<uint4 *>(to + 8 * q * kStepK) = y;
         }
       }
     };
@@ -551,7 +572,7 @@ struct StoreArgs {
   float *part;             // or float32 sums of each split, [splits, part_stride], added to what is there
   int64_t part_stride;
   int32_t accumulate;
-  int32_t wide;            // 16-bit out: four elements per store (its alignment and the row length allow it)
+  int32_t wide;            // 16-bit out: elements per store that its alignment and the row length allow: 8, 4 or 0 (single ones)
 };
 
 // kPartial: the sums go to a.part for join_kernel, else rounded to a.out.  kTurnA: operand a is turned.
@@ -574,14 +595,23 @@ __global__ __launch_bounds__(Tile::kThreads) void product_kernel(StoreArgs a) {
         for (int q = 0; q < 4; ++q) {
           const int64_t m = m0 + tile_row<Tile, kTurnA>(i, acc_row(4 * q, lane) + lane % 4);
           const bool zero = m < M && a.keep && a.keep[m] < 0;
+          static_assert(Tile::TN == 2, "a wave's columns are a line");
+          uint2 x[2];
 #pragma unroll
-          for (int j = 0; j < Tile::TN; ++j) {
-            uint2 x;
-            x.x = bits_of(acc.c[i][j][4 * q]) | bits_of(acc.c[i][j][4 * q + 1]) << 16;
-            x.y = bits_of(acc.c[i][j][4 * q + 2]) | bits_of(acc.c[i][j][4 * q + 3]) << 16;
-            x = turn4(x, lane);
-            const int64_t n = n0 + 32 * j + lane % 32 / 4 * 4;
-            if (m < M && n < N) *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + m * N + n) = zero ? uint2{0, 0} : x;
+          for (int j = 0; j < 2; ++j) {
+            x[j].x = bits_of(acc.c[i][j][4 * q]) | bits_of(acc.c[i][j][4 * q + 1]) << 16;
+            x[j].y = bits_of(acc.c[i][j][4 * q + 2]) | bits_of(acc.c[i][j][4 * q + 3]) << 16;
+            x[j] = turn4(x[j], lane);
+          }
+          uint4 y = line_of(x[0], x[1], lane);
+          if (zero) y = uint4{0, 0, 0, 0};
+          const int64_t n = n0 + line_column(lane);
+          uint16_t *to = static_cast<uint16_t *>(a.out) + m * N + n;
+          if (a.wide == 8) {
+            if (m < M && n < N) *reinterpret_cast<uint4 *>(to) = y;
+          } else {
+            if (m < M && n < N) *reinterpret_cast<uint2 *>(to) = uint2{y.x, y.y};
+            if (m < M && n + 4 < N) *reinterpret_cast<uint2 *>(to + 4) = uint2{y.z, y.w};
           }
         }
       return;
@@ -969,7 +999,7 @@ int forward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const Id *l
 template <typename T, bool kTurnA>
 int product(TileKind kind, StoreArgs a, T *out, bool partial, hipStream_t stream) {
   a.out = out;
-  a.wide = a.g.b.rows % 4 == 0 && aligned_to(out, 8);
+  a.wide = a.g.b.rows % 8 == 0 && aligned_to(out, 16) ? 8 : a.g.b.rows % 4 == 0 && aligned_to(out, 8) ? 4 : 0;
   return with_tile(kind, &a.g, [&](auto tile, dim3 grid) {
     using Tile = decltype(tile);
     if (partial)
