@@ -255,31 +255,55 @@ struct RunArgs {
   int32_t V, D;
   int lpr, accumulate;
   int fill_blocks;      // workgroups ahead of the others that write zeros into the absent rows
+  int fill_rows, fill_lpr;  // rows per wave of these, lanes per row (0: ranges)
   float scale;
   float *part;          // [2 * chunks, D] partial rows, slots 2c and 2c + 1 for the first and last run of chunk c
   int32_t *part_keys;   // [2 * chunks]
 };
 
-// Zeros in the rows that no id names.  A wave looks 64 rows up in the sorted ids (one binary search per lane), then
-// writes those of them that are absent.
-template <typename T, int VEC>
-__device__ __forceinline__ void zero_absent(const int2 *sorted, int32_t n, int32_t V, int32_t D, int lpr, T *grad) {
-  using P = Pack<T, VEC>;
-  const int lane = threadIdx.x & (kWaveSize - 1), sub = lane & (lpr - 1);
-  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWaveSize) * kWaveSize;
-  if (r0 >= V) return;
-  int32_t lo = 0, hi = n;
+// Zeros in the rows that no id names.  A wave looks `fill_rows` rows up in the sorted ids (one binary search per lane),
+// then writes those of them that are absent: row by row where rows are whole 16-byte pieces of memory, else neighbouring
+// absent rows as one range, whose pieces are whole but for the first and the last.
+template <typename T>
+__device__ __forceinline__ void zero_absent(const RunArgs &a, T *grad) {
+  const int lane = threadIdx.x & (kWaveSize - 1);
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * kWavesPerBlock + threadIdx.x / kWaveSize) * a.fill_rows;
+  if (r0 >= a.V) return;
+  const int32_t n = static_cast<int32_t>(a.n);
+  const bool asks = lane < a.fill_rows && r0 + lane < a.V;
+  int32_t lo = 0, hi = asks ? n : 0;
   while (lo < hi) {
     const int32_t m = lo + (hi - lo) / 2;
-    if (sorted[m].x < r0 + lane) lo = m + 1; else hi = m;
+    if (a.sorted[m].x < r0 + lane) lo = m + 1; else hi = m;
   }
-  const uint64_t present = __ballot(lo < n && sorted[lo].x == r0 + lane);
-  P z;
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) z.v[k] = narrow<T>(0.0f);
-  for (int r = lane / lpr; r < kWaveSize && r0 + r < V; r += kWaveSize / lpr) {
-    if ((present >> r) & 1) continue;
-    for (int32_t c = sub * VEC; c < D; c += lpr * VEC) *reinterpret_cast<P *>(grad + (r0 + r) * D + c) = z;
+  uint64_t absent = __ballot(asks && !(lo < n && a.sorted[lo].x == r0 + lane));
+  constexpr int64_t kPiece = 16 / sizeof(T);
+  if (a.fill_lpr) {
+    const int sub = lane & (a.fill_lpr - 1);
+    for (int r = lane / a.fill_lpr; r < a.fill_rows; r += kWaveSize / a.fill_lpr) {
+      if (!((absent >> r) & 1)) continue;
+      for (int64_t c = (static_cast<int64_t>(blockIdx.y) * a.fill_lpr + sub) * kPiece; c < a.D;
+           c += static_cast<int64_t>(gridDim.y) * a.fill_lpr * kPiece)
+        *reinterpret_cast<uint4 *>(grad + (r0 + r) * a.D + c) = uint4{0, 0, 0, 0};
+    }
+    return;
+  }
+  const int64_t ahead = reinterpret_cast<uintptr_t>(grad) % 16 / sizeof(T);  // elements between a 16-byte boundary and grad
+  while (absent) {
+    const int start = __ffsll(static_cast<unsigned long long>(absent)) - 1;
+    const uint64_t others = ~(absent >> start);
+    const int rows = others ? __ffsll(static_cast<unsigned long long>(others)) - 1 : kWaveSize;
+    absent = start + rows < kWaveSize ? absent >> (start + rows) << (start + rows) : 0;
+    const int64_t first = (r0 + start) * a.D, last = first + static_cast<int64_t>(rows) * a.D;
+    const int64_t begin = (first + ahead) / kPiece * kPiece - ahead;
+    for (int64_t c = begin + (static_cast<int64_t>(blockIdx.y) * kWaveSize + lane) * kPiece; c < last;
+         c += static_cast<int64_t>(gridDim.y) * kWaveSize * kPiece) {
+      if (c >= first && c + kPiece <= last) {
+        *reinterpret_cast<uint4 *>(grad + c) = uint4{0, 0, 0, 0};
+      } else {
+        for (int64_t k = max(c, first); k < min(c + kPiece, last); ++k) grad[k] = narrow<T>(0.0f);
+      }
+    }
   }
 }
 
@@ -287,7 +311,7 @@ __device__ __forceinline__ void zero_absent(const int2 *sorted, int32_t n, int32
 template <typename S, typename T, int VEC, bool kFirst>
 __global__ __launch_bounds__(kBlockThreads) void run_sums_kernel(RunArgs a, const S *rows, T *grad) {
   if (static_cast<int>(blockIdx.x) < a.fill_blocks) {
-    if (blockIdx.y == 0) zero_absent<T, VEC>(a.sorted, static_cast<int32_t>(a.n), a.V, a.D, a.lpr, grad);
+    zero_absent(a, grad);
     return;
   }
   constexpr int kAhead = 8;  // rows under way per lane
@@ -409,6 +433,7 @@ int radix_items(int64_t n) { return n <= 524288 ? 1024 : 4096; }
 int32_t chunk_of(int64_t n) { return n <= 8192 ? 4 : n <= 65536 ? 8 : n <= 524288 ? 16 : 64; }
 constexpr int32_t kNextChunk = 8;    // ... on the levels after it
 constexpr int64_t kJoinMost = 2048;  // partial rows that one group may have to join at the end (all ids equal)
+constexpr int64_t kFillWaves = 512;  // below which a wave takes fewer rows to zero
 constexpr int kMostLevels = 14;      // each leaves a quarter of the partial rows
 
 struct GradLayout {
@@ -500,7 +525,14 @@ int grad_rows(const int2 *sorted, int64_t n, int64_t V, int64_t D, const T *dout
   a.lpr = lpr;
   a.accumulate = accumulate;
   a.scale = scale;
-  a.fill_blocks = accumulate ? 0 : static_cast<int>((V + kWaveSize * kWavesPerBlock - 1) / (kWaveSize * kWavesPerBlock));
+  // a wave takes 64 rows, fewer where that leaves few waves: more waves search longer than they write (with 512, 1024 and
+  // 2048 as the limit: 4 ids into 104,121 x 201 float16 13.6, 14.0, 16.3 us; 13,978 into 48,525 x 161 bfloat16 51, 54, 55;
+  // 2 into 1105 x 971 float16 13 with each, 40 with 64 rows a wave and stores of single elements)
+  a.fill_rows = kWaveSize;
+  while (a.fill_rows > 4 && V < a.fill_rows * kFillWaves) a.fill_rows /= 4;
+  a.fill_lpr = VEC * sizeof(T) == 16 ? lpr : 0;
+  const int64_t fill_rows = static_cast<int64_t>(a.fill_rows) * kWavesPerBlock;
+  a.fill_blocks = accumulate ? 0 : static_cast<int>((V + fill_rows - 1) / fill_rows);
   const float *rows = nullptr;
   for (int k = 0; k < g.levels; ++k) {
     a.chunk = k ? kNextChunk : chunk_of(n);

@@ -254,3 +254,32 @@ def test_bad_arguments_of_the_entry_points_without_a_device():
     assert L.fg_embedding_grad(4, 4, 100, 8, 8, 8, 1.0, 0, 0, 0, 264, small, None) == -1   # not at a multiple of 256
     assert L.fg_embedding_grad(4, 4, 100, 8, None, 8, 1.0, 0, 0, 0, 256, small, None) == -1
     assert L.fg_embedding_grad(4, 4, 0, None, None, None, 1.0, 1, 0, 0, None, 0, None) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("V,D", [(40000, 3), (40000, 8), (9001, 5), (700, 33), (700, 32), (63, 1), (1, 7)])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_absent_rows_become_zeros_and_nothing_beside_them(dtype, V, D, offset):
+    """Rows that no id names, alone, in pairs and in long ranges, of a gradient that begins `offset` elements past an
+    aligned address, between guards.  Every id is named once, so each sum is one element and the result exact."""
+    L = _lib.lib()
+    t = getattr(torch, dtype)
+    patterns = [torch.tensor([V // 2]), torch.arange(0, V, 2), torch.arange(0, V, 3), torch.arange(max(1, V - 70)),
+                torch.tensor([0, V - 1][:V]), torch.arange(V)]
+    for pattern in patterns:
+        ids = pattern.to("cuda", torch.int32)
+        n = ids.numel()
+        dout = torch.arange(1, n * D + 1, device="cuda").remainder(97).add(1).to(t).reshape(n, D)
+        buf = torch.full((offset + V * D + 24,), float("nan"), device="cuda", dtype=t)
+        need = ctypes.c_int64(0)
+        assert L.fg_embedding_grad_workspace(V, D, n, ctypes.byref(need)) == 0
+        space = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+        grad = buf[offset:offset + V * D]
+        assert L.fg_embedding_grad(V, D, n, ids.data_ptr(), dout.data_ptr(), grad.data_ptr(), 1.0, 0,
+                                   {"float32": 0, "float16": 2}[dtype], 0, space.data_ptr(), need.value,
+                                   torch.cuda.current_stream().cuda_stream) == 0
+        want = torch.zeros(V, D, device="cuda", dtype=t)
+        want[ids.long()] = dout
+        assert torch.equal(grad.reshape(V, D), want)
+        assert buf[:offset].isnan().all() and buf[offset + V * D:].isnan().all()
