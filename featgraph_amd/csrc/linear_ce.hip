@@ -10,7 +10,8 @@
 // Backward: the logits are computed again piece by piece of the vocabulary; the epilogue turns them into P, and two
 // more products over P give the piece's rows of dw and its share of dh.  P is stored once, as [v, n]: dw's product reads
 // its rows, dh's its columns (mfma_gemm.hpp).  h and w are transposed into copies for these products (2 N D + 2 V D
-// elements of traffic against 6 N V D flops); the copy of h also holds zeros in place of the rows to ignore.
+// elements of traffic against 6 N V D flops), bfloat16 rows that have to be padded in the same pass (19 rows x 137,737 classes
+// x 89: 103 -> 76 us); the copy of h also holds zeros in place of the rows to ignore.
 //
 // Where it stands (bfloat16): 4096 rows x 65,536 classes x 1024: statistics 463 us (1188 TFLOP/s), P 590, the two products
 // 490 each; a library's product of 8192^3 reaches 1333.  1024 x 232,965 x 128: statistics 82 us (745 TFLOP/s), where the
@@ -99,6 +100,7 @@ struct CopyJob {
                             // (null: not wanted), read by the transposed copy
   const int32_t *keep;      // rows whose keep[] is negative do not count in peak, and are zeros in the transposed copy
   const float *factor;      // float32: per row, for peak and the transposed copy (null: 1)
+  uint16_t *rows_out;       // bfloat16, transposed copy: where the row copy goes, made in the same pass (null: not wanted)
 };
 struct CopyJobs {
   CopyJob job[2];
@@ -110,15 +112,29 @@ __device__ __forceinline__ const CopyJob &job_of(const CopyJobs &jobs, uint32_t 
   return jobs.job[second];
 }
 
-// bfloat16: [rows, D] -> panels
+// kVec elements from any address of theirs on; past the row's end zeros.
+template <typename T, int kVec>
+__device__ __forceinline__ Pack<T, kVec> load_within(const T *row, int64_t c, int32_t D) {
+  Pack<T, kVec> v;
+  if (c + kVec <= D) {
+    __builtin_memcpy(&v, row + c, sizeof(v));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v.v[j] = c + j < D ? row[c + j] : T{};
+  }
+  return v;
+}
+
+// bfloat16: [rows, D] -> panels, eight elements per lane
 __device__ __forceinline__ void pad_rows(const CopyJob &job, uint32_t block) {
+  constexpr int kPieces = kStepK / 8;  // of a row in a panel
   const auto *x = static_cast<const uint16_t *>(job.x);
-  const int64_t per_panel = job.rows * kStepK;
+  const int64_t per_panel = job.rows * kPieces;
   const int64_t total = per_panel * ((job.D + kStepK - 1) / kStepK), stride = static_cast<int64_t>(job.blocks) * kBlockThreads;
   for (int64_t t = static_cast<int64_t>(block) * kBlockThreads + threadIdx.x; t < total; t += stride) {
     const int64_t panel = t / per_panel, in_panel = t - panel * per_panel;
-    const int64_t c = panel * kStepK + in_panel % kStepK;
-    job.out[t] = c < job.D ? x[in_panel / kStepK * job.D + c] : 0;
+    *reinterpret_cast<Pack<uint16_t, 8> *>(job.out + t * 8) =
+        load_within<uint16_t, 8>(x + in_panel / kPieces * job.D, panel * kStepK + in_panel % kPieces * 8, job.D);
   }
 }
 
@@ -190,10 +206,10 @@ __global__ __launch_bounds__(kBlockThreads) void copy_rows_kernel(CopyJobs jobs)
 
 // [rows, D] -> parts of its transpose as panels of 64 rows' elements, zeros in place of rows whose keep[] is negative
 // (whatever those hold must not reach the sum over rows).  float32: times factor[row] and brought into range by *peak.
-// 64 x 64 elements per workgroup, 16 bytes per lane on both sides where D allows (kVec elements per load).
-template <typename T, int kVec>
+// 64 x 64 elements per workgroup, 16 bytes per lane on both sides.
+template <typename T>
 __global__ __launch_bounds__(kBlockThreads) void copy_transposed_kernel(CopyJobs jobs) {
-  constexpr int kLanes = 64 / kVec;  // per row
+  constexpr int kVec = 16 / sizeof(T), kLanes = 64 / kVec;  // per row
   __shared__ float tile[64][65];
   uint32_t block;
   const CopyJob &job = job_of(jobs, &block);
@@ -206,8 +222,8 @@ __global__ __launch_bounds__(kBlockThreads) void copy_transposed_kernel(CopyJobs
   for (int k = threadIdx.x / kLanes; k < 64; k += kBlockThreads / kLanes) {
     const int64_t r = r0 + k;
     Pack<T, kVec> v;
-    const bool there = r < job.rows && c < D && (!job.keep || job.keep[r] >= 0);
-    if (there) v = *reinterpret_cast<const Pack<T, kVec> *>(static_cast<const T *>(job.x) + r * D + c);
+    const bool there = r < job.rows && (!job.keep || job.keep[r] >= 0);
+    if (there) v = load_within<T, kVec>(static_cast<const T *>(job.x) + r * D, c, D);
     const float f = sizeof(T) == 4 && there && job.factor ? job.factor[r] : 1.0f;
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
@@ -226,6 +242,17 @@ __global__ __launch_bounds__(kBlockThreads) void copy_transposed_kernel(CopyJobs
 #pragma unroll
       for (int k = 0; k < 8; ++k) y.v[k] = static_cast<uint16_t>(part_of<T>(tile[8 * g + k][col], p));
       *reinterpret_cast<Pack<uint16_t, 8> *>(job.out + ((panel + p * panels) * D + c0 + col) * kStepK + 8 * g) = y;
+    }
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (job.rows_out == nullptr) return;
+    for (int t = threadIdx.x; t < 512; t += kBlockThreads) {  // eight columns of one row each
+      const int g = t % 8, k = t / 8;
+      if (r0 + k >= job.rows) continue;
+      Pack<uint16_t, 8> y;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y.v[j] = static_cast<uint16_t>(bits_of(tile[k][8 * g + j]));
+      *reinterpret_cast<Pack<uint16_t, 8> *>(job.rows_out + panel_at(job.rows, r0 + k, c0 + 8 * g)) = y;
     }
   }
 }
@@ -947,30 +974,24 @@ void copy_rows(CopyJobs jobs, hipStream_t stream) {
   for (CopyJob &j : jobs.job)
     j.blocks = j.rows == 0 ? 0
                : sizeof(T) == 4 ? static_cast<uint32_t>(std::min<int64_t>((j.rows + kWavesPerBlock - 1) / kWavesPerBlock, 4096))
-                                : flat_grid(panel_elements(j.rows, j.D));
+                                : flat_grid(panel_elements(j.rows, j.D) / 8);
   const dim3 grid(jobs.job[0].blocks + jobs.job[1].blocks);
   const int64_t D = std::max(jobs.job[0].D, jobs.job[1].D);
-  if (sizeof(T) == 2 || D > 16 * kWaveSize)
-    copy_rows_kernel<T, 0><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
-  else if (D > 8 * kWaveSize)
-    copy_rows_kernel<T, 16><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
-  else if (D > 2 * kWaveSize)
-    copy_rows_kernel<T, 8><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
-  else
-    copy_rows_kernel<T, 2><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
+  auto launch = [&](auto held) {
+    copy_rows_kernel<T, decltype(held)::value><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
+  };
+  if constexpr (sizeof(T) == 2) launch(std::integral_constant<int, 0>{});
+  else if (D > 16 * kWaveSize) launch(std::integral_constant<int, 0>{});
+  else if (D > 8 * kWaveSize) launch(std::integral_constant<int, 16>{});
+  else if (D > 2 * kWaveSize) launch(std::integral_constant<int, 8>{});
+  else launch(std::integral_constant<int, 2>{});
 }
 
 template <typename T>
 void copy_transposed(CopyJobs jobs, hipStream_t stream) {
-  constexpr int kVec = 16 / sizeof(T);
-  bool wide = true;
-  for (CopyJob &j : jobs.job) {
-    j.blocks = static_cast<uint32_t>(steps_of(j.rows) * ((j.D + 63) / 64));
-    wide = wide && (j.rows == 0 || (j.D % kVec == 0 && aligned_to(j.x, 16)));
-  }
+  for (CopyJob &j : jobs.job) j.blocks = static_cast<uint32_t>(steps_of(j.rows) * ((j.D + 63) / 64));
   const dim3 grid(jobs.job[0].blocks + jobs.job[1].blocks);
-  if (wide) copy_transposed_kernel<T, kVec><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
-  else copy_transposed_kernel<T, 1><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
+  copy_transposed_kernel<T><<<grid, dim3(kBlockThreads), 0, stream>>>(jobs);
 }
 
 template <typename T>
@@ -1066,6 +1087,8 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
   rows_of.job[0] = CopyJob{h, reinterpret_cast<uint16_t *>(ws + l.h_pack), N, static_cast<int32_t>(D), 0, h_exp, peaks, label, factor};
   transposed.job[0] = rows_of.job[0];
   transposed.job[0].out = ht;
+  const bool together = sizeof(T) == 2 && l.packed;  // both copies in one pass
+  if (together) transposed.job[0].rows_out = rows_of.job[0].out;
   a.g.b = operand<T>(rows_of.job[0], l);
   const bool dh_partial = l.dh_splits > 1 || V > l.piece;
   JoinJobs joins{};
@@ -1077,8 +1100,9 @@ int backward(int64_t N, int64_t V, int64_t D, const T *h, const T *w, const floa
     rows_of.job[1] = CopyJob{w + v0 * D, reinterpret_cast<uint16_t *>(ws + l.w_pack), rows, static_cast<int32_t>(D), 0, w_exp, peak};
     transposed.job[1] = rows_of.job[1];
     transposed.job[1].out = wt;
+    if (together) transposed.job[1].rows_out = rows_of.job[1].out;
     a.g.a = operand<T>(rows_of.job[1], l);
-    if (l.packed) copy_rows<T>(rows_of, stream);
+    if (l.packed && !together) copy_rows<T>(rows_of, stream);
     copy_transposed<T>(transposed, stream);
     rows_of.job[0].rows = transposed.job[0].rows = 0;  // h is there now
     int rc = with_tile(l.logits, &a.g, [&](auto tile, dim3) {
