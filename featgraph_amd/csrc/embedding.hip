@@ -20,7 +20,7 @@
 namespace fg {
 namespace {
 
-constexpr int kRankSortMost = 16384;  // ids that the one-launch sort takes (64 KB of LDS)
+constexpr int kRankSortMost = 12288;  // ids that the one-launch sort takes (48 KB of LDS)
 constexpr int kRankThreads = 1024;
 constexpr int kRadixBits = 11;        // most bits per pass
 constexpr int32_t kSkip = INT32_MIN;  // flag on a partial row's key: nothing there to add
@@ -71,8 +71,8 @@ __global__ __launch_bounds__(kBlockThreads) void lookup_kernel(const T *table, c
 // ------------------------------------------------------------------------------------------------ sort
 // Up to kRankSortMost ids: the place of id i is the number of ids below it plus the number of equal ids before it,
 // counted directly.  A workgroup holds all ids in LDS and places 64 of them; each of its 16 waves counts over a
-// sixteenth of the list, four ids per LDS read.  N * N / 64 wave steps, but one launch (5 us for 333 ids, 20 for 16384,
-// where the six launches of the radix sort take 30).
+// sixteenth of the list, four ids per LDS read.  N * N / 64 wave steps, but one launch: whole gradients take 26, 37,
+// 44 and 49 us for 4100, 10000, 13978 and 16384 ids where those with the six launches of the radix sort take 41, 42, 43 and 43.
 template <typename Id>
 __global__ __launch_bounds__(kRankThreads) void rank_sort_kernel(const Id *ids, int32_t n, int32_t V, int2 *sorted) {
   constexpr int kWaves = kRankThreads / kWaveSize;

@@ -13,9 +13,9 @@
 // elements of traffic against 6 N V D flops), bfloat16 rows that have to be padded in the same pass (19 rows x 137,737 classes
 // x 89: 103 -> 76 us); the copy of h also holds zeros in place of the rows to ignore.
 //
-// Where it stands (bfloat16): 4096 rows x 65,536 classes x 1024: statistics 463 us (1188 TFLOP/s), P 590, the two products
-// 490 each; a library's product of 8192^3 reaches 1333.  1024 x 232,965 x 128: statistics 82 us (745 TFLOP/s), where the
-// epilogue's exponentials count as much as the products.
+// Where it stands (bfloat16), whole calls: 4096 rows x 65,536 classes x 1024: loss 450 us (1222 TFLOP/s), gradient 1512 (its
+// three products: 1091); a library's product of 8192^3 reaches 1333.  1024 x 232,965 x 128: 88 and 446, bound by the
+// epilogues: an exponential per logit, P written once and read twice.
 //
 // Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step of each
 // term, random in sign; the results are rounded to bfloat16 themselves); everything between is float32.  float32

@@ -283,3 +283,20 @@ def test_absent_rows_become_zeros_and_nothing_beside_them(dtype, V, D, offset):
         want[ids.long()] = dout
         assert torch.equal(grad.reshape(V, D), want)
         assert buf[:offset].isnan().all() and buf[offset + V * D:].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("index", ["int32", "int64"])
+@pytest.mark.parametrize("n", [12287, 12288, 12289, 12353])
+@pytest.mark.parametrize("V", [1, 500, 70000])
+def test_gradient_around_the_border_of_the_two_sorts(n, V, index):
+    """Whole numbers below 2^24 in every sum, so that float32 holds each exactly whatever the order."""
+    rng = np.random.default_rng(n + V)
+    ids = rng.integers(-1, V, n)
+    dout = rng.integers(-8, 9, (n, 3)).astype(np.float32)
+    g = EmbeddingLookupGradhip()
+    g.build([placeholder((V, 3)), placeholder((n,), index)])
+    got = g.run([torch.from_numpy(ids).to("cuda", getattr(torch, index)), torch.from_numpy(dout).cuda()]).asnumpy()
+    want = np.zeros((V, 3), np.float64)
+    np.add.at(want, ids[ids >= 0], dout[ids >= 0])
+    assert np.array_equal(got, want.astype(np.float32))
