@@ -342,3 +342,35 @@ def test_pieces_stay_within_32_bit_offsets(dtype):
     finally:
         _lib.config_set("ce.piece_rows", 0)
     assert len(set(sizes)) == 1, sizes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("D", [128, 67, 100])
+@pytest.mark.parametrize("tile,piece", [(0, 0), (1, 256), (2, 256), (3, 512), (4, 256)])
+def test_ignored_rows_in_every_path(dtype, D, tile, piece):
+    """Operands read in place, padded and with rows of odd length; one piece and several; infinities beside NaN."""
+    N, V = 150, 700
+    h, w, y, dl = _operands(dtype, N, V, D, 11, ignored=0.3)
+    bad = (y < 0) | (y >= V)
+    try:
+        _lib.config_set("ce.tile", tile)
+        _lib.config_set("ce.piece_rows", piece)
+        ph = [placeholder((N, D), dtype), placeholder((V, D), dtype), placeholder((N,), "int32")]
+        f, g = LinearCrossEntropyhip(), LinearCrossEntropyGradhip()
+        f.build(ph), g.build(ph)
+        _, lse = (x.tensor.clone() for x in f.run([h, w, y]))
+        dh, dw = (x.tensor.clone() for x in g.run([h, w, y, lse, dl]))
+        assert bool(bad.any()) and dh.isfinite().all() and dw.isfinite().all()
+        h[bad] = float("nan")
+        h[bad, ::2] = float("inf")
+        lse[bad], dl[bad] = float("nan"), float("-inf")
+        loss2, _ = f.run([h, w, y])
+        assert not loss2.tensor[bad].any() and loss2.tensor.isfinite().all()
+        dh2, dw2 = g.run([h, w, y, lse, dl])
+        assert torch.equal(dh2.tensor, dh) and torch.equal(dw2.tensor, dw) and not dh2.tensor[bad].any()
+        w[5] = float("inf")                             # a class that spoils every row it meets, but not the ignored ones
+        assert not g.run([h, w, y, lse, dl])[0].tensor[bad].any()
+    finally:
+        _lib.config_set("ce.tile", 0)
+        _lib.config_set("ce.piece_rows", 0)
