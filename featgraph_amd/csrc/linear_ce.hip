@@ -344,13 +344,13 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   const int wm = wave / Tile::WN, wn = wave % Tile::WN;
   const int64_t n0 = static_cast<int64_t>(at.tn) * Tile::BN + wn * (Tile::BN / Tile::WN);
   const int64_t first_v = static_cast<int64_t>(at.tm) * Tile::BM + wm * (Tile::BM / Tile::WM);
-  float top[Tile::TN], sum[Tile::TN];
+  float top[Tile::TN], sum[Tile::TN], rest[Tile::TN];  // the sum is sum + rest
   int64_t label[Tile::TN];  // row of the piece that is the label's, relative to this wave's first
 #pragma unroll
   for (int j = 0; j < Tile::TN; ++j) {
     const int64_t n = n0 + 32 * j + lane % 32;
     top[j] = -INFINITY;
-    sum[j] = 0.0f;
+    sum[j] = rest[j] = 0.0f;
     label[j] = n < a.g.b.rows ? static_cast<int64_t>(static_cast<const Id *>(a.labels)[n]) - a.v0 - first_v : -1;
   }
   gemm_tiles<Tile, M, false>(a.g, at, tiles, lds, acc, [&](int tile) {
@@ -384,19 +384,29 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
         for (int r = 0; r < 16; ++r) m = fmaxf(m, acc.c[i][j][r]);
       m = fmaxf(top[j], __builtin_ceilf(m * kLog2e));
       const float from = m == -INFINITY ? 0.0f : m;
-      float s = sum[j] * __builtin_amdgcn_exp2f(top[j] - from);
+      // The tile's terms: 16 one by one, then the sums of 16.
+      float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < Tile::TM; ++i)
+      for (int i = 0; i < Tile::TM; ++i) {
+        float t = 0.0f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][r], kLog2e, -from));
+        for (int r = 0; r < 16; ++r) t += __builtin_amdgcn_exp2f(__builtin_fmaf(acc.c[i][j][r], kLog2e, -from));
+        s += t;
+      }
+      // Added to the sum of the tiles before, what the addition rounds off to the rest: a range may have thousands of
+      // tiles, each of them small against the sum.
+      const float times = __builtin_amdgcn_exp2f(top[j] - from), old = sum[j] * times;
+      sum[j] = old + s;
+      const float added = sum[j] - old;
+      rest[j] = rest[j] * times + ((old - (sum[j] - added)) + (s - added));
       top[j] = m;
-      sum[j] = s;
     }
     clear(acc);
   });
   float2 *stats = reinterpret_cast<float2 *>(lds);  // [WM][BN]
 #pragma unroll
   for (int j = 0; j < Tile::TN; ++j) {
+    sum[j] += rest[j];
     const float2 s = join_stats(float2{top[j], sum[j]},
                                 float2{__shfl_xor(top[j], 32, kWaveSize), __shfl_xor(sum[j], 32, kWaveSize)});
     if (lane < 32) stats[wm * Tile::BN + wn * (Tile::BN / Tile::WN) + 32 * j + lane] = s;
@@ -412,28 +422,41 @@ __global__ __launch_bounds__(Tile::kThreads) void stats_kernel(StatsArgs a) {
   }
 }
 
-// kShares threads per row share its ranges.  `loss` holds the label's logits on entry.
+// kShares threads per row share its ranges, whose sums are added in double.  `loss` holds the label's logits on entry.
 constexpr int kFewRanges = 8;
 template <typename Id, int kShares>
 __global__ __launch_bounds__(kBlockThreads) void loss_kernel(const float2 *part, int32_t ranges, const Id *labels,
                                                              int32_t N, int64_t V, float *loss, float *lse) {
   constexpr int kRows = kBlockThreads / kShares;
-  __shared__ float2 joined[kShares][kRows];
+  struct Sum {
+    double s;
+    float r;  // whole, of s * 2^r
+  };
+  auto join = [](const Sum &a, const Sum &b) {
+    const float r = fmaxf(a.r, b.r);
+    if (r == -INFINITY) return Sum{a.s + b.s, r};
+    auto down = [r](const Sum &x) { return ldexp(x.s, static_cast<int>(fmaxf(x.r - r, -2000.0f))); };  // 0 beyond 2^-1074
+    return Sum{down(a) + down(b), r};
+  };
+  __shared__ Sum joined[kShares][kRows];
   const int row = threadIdx.x % kRows, share = threadIdx.x / kRows;
   const int64_t n = static_cast<int64_t>(blockIdx.x) * kRows + row;
-  float2 s{-INFINITY, 0.0f};
+  Sum s{0.0, -INFINITY};
   if (n < N)
-    for (int32_t t = share; t < ranges; t += kShares) s = join_stats(s, part[static_cast<int64_t>(t) * N + n]);
+    for (int32_t t = share; t < ranges; t += kShares) {
+      const float2 x = part[static_cast<int64_t>(t) * N + n];
+      s = join(s, Sum{x.y, x.x});
+    }
   if constexpr (kShares > 1) {
     joined[share][row] = s;
 #pragma unroll
     for (int half = kShares / 2; half > 0; half >>= 1) {
       __syncthreads();
-      if (share < half) joined[share][row] = s = join_stats(s, joined[share + half][row]);
+      if (share < half) joined[share][row] = s = join(s, joined[share + half][row]);
     }
   }
   if (share == 0 && n < N) {
-    const float r = static_cast<float>((static_cast<double>(s.x) + log2(static_cast<double>(s.y))) * 0.69314718055994530942);
+    const float r = static_cast<float>((static_cast<double>(s.r) + log2(s.s)) * 0.69314718055994530942);
     const Id y = labels[n];
     lse[n] = r;
     loss[n] = y >= 0 && static_cast<int64_t>(y) < V ? r - loss[n] : 0.0f;

@@ -374,3 +374,54 @@ def test_ignored_rows_in_every_path(dtype, D, tile, piece):
     finally:
         _lib.config_set("ce.tile", 0)
         _lib.config_set("ce.piece_rows", 0)
+
+
+# One range of the vocabulary per workgroup, and as many ranges as there are tiles: the sums of exponentials are long.
+LONG_RANGES = [("bfloat16", tile, 0, -1, 65536) for tile in (0, 1, 2, 3, 4)] + \
+              [("float32", tile, 0, native, 65536) for tile in (1, 2, 3, 4) for native in (0, 1)] + \
+              [(dtype, 0, 256, -1, 40) for dtype in TYPES]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("place", ["flat", "first", "last"])
+@pytest.mark.parametrize("dtype,tile,piece,native,N", LONG_RANGES)
+def test_sums_over_a_long_vocabulary(config, dtype, tile, piece, native, N, place):
+    """232,965 classes of one logit c (whose exponential is no power of two), and the same with one class 17.75 above the
+    others, whose term alone is larger than 2^24 of theirs: lse = c + log(V) and c + log(V - 1 + e^17.75).
+
+    Sixteen terms are added one by one and four such sums together (18 roundings), the running sum is two floats that are
+    put together once, halves of a wave and four waves make four more, exp2 is off by a step (2 halves), its argument by
+    the rounding of log2(e) (1.4e-8 |l| log2(e), with |l| below 19 less than 5 halves) and its own (|argument| at most 1
+    for the terms that count): below 32 * 2^-24 together.  The result is rounded to float32."""
+    V, peak = 232965, 17.75
+    config("ce.tile", tile)
+    config("ce.piece_rows", piece)
+    config("ce.native", native)
+    h = torch.ones(N, 2, dtype=TYPES[dtype], device="cuda")
+    h[:, 0] = 0.296875 + (torch.arange(N, device="cuda") % 8) / 16.0
+    w = torch.zeros(V, 2, dtype=TYPES[dtype], device="cuda")
+    w[:, 0] = 1.0
+    at = V - 1 if place == "last" else 0
+    w[at, 1] = 0.0 if place == "flat" else peak
+    y = torch.full((N,), at, dtype=torch.int32, device="cuda")
+    f = LinearCrossEntropyhip()
+    f.build([placeholder((N, 2), dtype), placeholder((V, 2), dtype), placeholder((N,), "int32")])
+    loss, lse = (x.tensor for x in f.run([h, w, y]))
+    c = h[:, 0].double()
+    top = math.exp(float(w[at, 1]))
+    want = c + math.log(V - 1 + top)
+    want_loss = torch.full_like(want, math.log(V - 1 + top) - float(w[at, 1]))
+    tol = 32 * 2.0 ** -24 + 1.01 * 2.0 ** -24 * want
+    assert bool(((lse.double() - want).abs() <= tol).all())
+    assert bool(((loss.double() - want_loss).abs() <= tol + 2.0 ** -24 * want_loss).all())
+
+    # the label's gradient, p - 1, of a few rows with the lse of all: p is off by p times the errors of lse, the logit's
+    # and exp2's (16 * 2^-24), G and the result are rounded to the type or to two parts
+    some = torch.arange(0, N, max(1, N // 40), device="cuda")
+    g = LinearCrossEntropyGradhip()
+    g.build([placeholder((some.numel(), 2), dtype), placeholder((V, 2), dtype), placeholder((some.numel(),), "int32")])
+    dl = torch.ones(some.numel(), device="cuda")
+    dh = g.run([h[some].contiguous(), w, y[some].contiguous(), lse[some].contiguous(), dl])[0].tensor
+    exact = float(w[at, 1]) * (top / (V - 1 + top) - 1)
+    off = float(w[at, 1]) * (tol[some] + 16 * 2.0 ** -24) + 4 * HALF_STEP[dtype] * abs(exact)
+    assert bool(((dh[:, 1].double() - exact).abs() <= off).all())
