@@ -937,7 +937,7 @@ Layout layout(int64_t N, int64_t V, int64_t D, int dtype, bool aligned, bool bac
     const TileSize *sizes = l.native ? kNativeSize : kTileSize;
     l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, s.stats, &l.ranges); }, sizes);
     choose_ranges(sizes[l.logits], in_piece, N, steps, sizes[l.logits].stats, &l.ranges);
-    l.stats = take(l.pieces * std::min<int64_t>(tiles_of(l.piece, kTileSize[l.logits].bm), kMostRanges) * N * 8);
+    l.stats = take(l.pieces * l.ranges * N * 8);
   } else {
     l.logits = choose_tile([&](const TileSize &s) { return choose_ranges(s, in_piece, N, steps, l.parts * s.grad, &l.ranges); });
     choose_ranges(kTileSize[l.logits], in_piece, N, steps, l.parts * kTileSize[l.logits].grad, &l.ranges);

@@ -425,3 +425,34 @@ def test_sums_over_a_long_vocabulary(config, dtype, tile, piece, native, N, plac
     exact = float(w[at, 1]) * (top / (V - 1 + top) - 1)
     off = float(w[at, 1]) * (tol[some] + 16 * 2.0 ** -24) + 4 * HALF_STEP[dtype] * abs(exact)
     assert bool(((dh[:, 1].double() - exact).abs() <= off).all())
+
+
+@pytest.mark.parametrize("N,V,D", [(232965, 65536, 64), (65536, 232965, 128), (2 ** 22, 65536, 64), (2449029, 232965, 128)])
+def test_workspace_of_the_loss_holds_what_the_kernels_write(N, V, D):
+    """Beside the padded copies of operands off their alignment there are a reference and a sum for every row and range of
+    the vocabulary.  With this many rows every workgroup slot of the device is busy several times over with a few ranges."""
+    need = ctypes.c_int64(0)
+    assert _lib.lib().fg_linear_ce_workspace(N, V, D, 1, ctypes.byref(need)) == 0
+    copies = 2 * (N + V) * D + 2 * 256 * D                    # the piece of the vocabulary is a multiple of 256 rows
+    assert need.value <= copies + 32 * 8 * N + 4096, (need.value - copies) / (8 * N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("tile,piece", [(0, 0), (1, 256), (2, 512), (3, 768), (4, 256)])
+@pytest.mark.parametrize("N,V,D", [(5, 3000, 16), (300, 1025, 64), (2000, 70, 33), (1, 1, 1), (64, 20000, 128), (9000, 1300, 64)])
+def test_nothing_is_written_behind_the_workspace(config, dtype, tile, piece, N, V, D):
+    config("ce.tile", tile)
+    config("ce.piece_rows", piece)
+    h, w, y, dl = _operands(dtype, N, V, D, N + V)
+    ph = [placeholder((N, D), dtype), placeholder((V, D), dtype), placeholder((N,), "int32")]
+    f, g = LinearCrossEntropyhip(), LinearCrossEntropyGradhip()
+    f.build(ph), g.build(ph)
+    for m in (f, g):
+        need, behind = m._space.numel(), 1 << 20
+        m._space = torch.full((need + behind,), 0x5a, dtype=torch.uint8, device="cuda")
+        if m is f:
+            _, lse = m.run([h, w, y])
+        else:
+            m.run([h, w, y, lse, dl])
+        assert bool((m._space[need:] == 0x5a).all())
