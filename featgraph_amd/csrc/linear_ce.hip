@@ -19,9 +19,12 @@
 //
 // Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step of each
 // term, random in sign; the results are rounded to bfloat16 themselves); everything between is float32.  float32
-// operands, P among them, are split into two float16 parts (mfma_gemm.hpp), which keeps float32's accuracy; the loss
-// multiplies them as they are where reading one of them bounds it (few rows, or few classes).  P is at
-// most 1 and stored times 2^14; dloss is applied to the rows of dh in the epilogue and to the copy of h for dw.
+// operands, P among them, are split into two float16 parts (mfma_gemm.hpp); the loss multiplies them as they are where
+// reading one of them bounds it (few rows, or few classes).  P is at most 1 and stored times 2^14; dloss is applied to the
+// rows of dh in the epilogue and to the copy of h for dw.  What the parts keep: x of a row (logits) or of a whole matrix
+// (transposed copies) with the largest element m to 2^-23 |x| + 2^-50 m, P to 2^-23 P + 2^-50; sums are rounded as if
+// every factor were at least 2^-28 of the largest.  Smaller probabilities and features than 2^-27 of the largest so lose
+// relative accuracy; a third part would keep them at twice the products.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -3,10 +3,11 @@
 //
 // bfloat16 operands are multiplied as they are.  A float32 operand comes as two float16 parts of x * 2^e: hi, the value
 // rounded to 11 bits, and lo, the rest times 2^11 rounded to 11 bits, so that hi + lo * 2^-11 is x * 2^e to 2^-23 of
-// itself (the exponent e of a row or a matrix brings its largest element to 2^14; elements down to 2^-28 of that keep
-// full relative accuracy, smaller ones 2^-49 of the largest).  Three of the four products are added: hi * lo and lo * hi
-// first, then, after the sum is multiplied by 2^-11, hi * hi; lo * lo is at most 2^-24 of the terms.  That is float32's
-// accuracy at a third of the 16-bit rate, 5.3 times the peak rate of the float32 matrix instructions.
+// itself (the exponent e of a row or a matrix brings its largest element to 2^14 or more; elements down to 2^-27 of that keep
+// their relative accuracy, smaller ones 2^-50 of the largest, and weigh like 2^-28 of it where the matrix instructions align
+// the products that they add: a denormal factor counts as 2^-14 there).  Three of the four products are added: hi * lo and lo * hi
+// first, then, after the sum is multiplied by 2^-11, hi * hi; lo * lo is at most 2^-22 of a term, of either sign.  That is
+// near float32's accuracy at a third of the 16-bit rate, 5.3 times the peak rate of the float32 matrix instructions.
 //
 // A workgroup computes a BM x BN tile in steps of 64 k.  The operands' rows go straight to LDS (16 bytes per lane, whole
 // 128-byte lines, no registers in between) into the next of two stages of B and, where LDS allows, three of A: then only

@@ -2,13 +2,18 @@
 
 Not in the reference, which stops at the features of the last layer.  Vertex classification scores every vertex
 against the class weights; link prediction scores a batch of queries against the embeddings of all vertices.  With N
-rows and V classes the logits are an N x V matrix that is far larger than the operands; here it is never stored:
+rows and V classes the logits are an N x V matrix that is far larger than the operands; the loss never stores it:
 
     l[n, v] = <Hidden[n], Weight[v]>        lse[n] = log(sum_v exp l[n, v])        Loss[n] = lse[n] - l[n, Label[n]]
     G[n, v] = dLoss[n] * (exp(l[n, v] - lse[n]) - [v = Label[n]])     dHidden = G Weight     dWeight = G^T Hidden
 
 A label outside [0, V) (such as -1) marks a row to ignore: its loss is zero, its row of dHidden is zero and it adds
 nothing to dWeight.  Operands are float32 or bfloat16, losses and statistics float32.
+
+The gradient keeps G for a piece of the vocabulary (all of it where that and the copies of the operands fit 4 GiB) in the
+module's workspace: 2 bytes per row and class for bfloat16, 4 for float32.  bfloat16 rounds G to bfloat16.  float32 keeps
+G / dLoss to 2^-23 of itself and 2^-50, and elements of Weight and of dLoss * Hidden to 2^-23 of themselves and 2^-50 of
+the matrix's largest: probabilities or features less than 2^-27 of the largest lose relative accuracy.
 """
 import torch
 

@@ -605,6 +605,12 @@ FG_API int fg_grad_clip(int32_t count, const fg_tensor *tensors, float max_norm,
  * for hidden [N, D] and weight [V, D] of float32 or bfloat16 (float16 returns
  * FG_EUNSUPPORTED).  Logits, statistics and results are float32.  Limits:
  * N <= 4194304, D <= 65536.
+ *
+ * float32 operands may be multiplied as two float16 parts: an element x of a
+ * row whose largest is m is then kept to 2^-23 |x| + 2^-50 m, a product of two
+ * elements to 2^-21 of itself, and float32 sums are rounded as if every element
+ * were at least 2^-28 m.  Infinite elements then make logits NaN, also where
+ * the formula has an infinity.
  */
 FG_API int fg_linear_ce_workspace(int64_t N, int64_t V, int64_t D, int32_t dtype, int64_t *bytes);
 FG_API int fg_linear_ce(int64_t N, int64_t V, int64_t D, const void *hidden, const void *weight, const void *labels,
@@ -618,8 +624,15 @@ FG_API int fg_linear_ce(int64_t N, int64_t V, int64_t D, const void *hidden, con
  *   dweight[v, :] = sum over n of G[n, v] * hidden[n, :]
  * Rows whose label is outside [0, V) get zeros in dhidden and add nothing to
  * dweight, whatever their hidden row, lse and dloss hold.  The logits are
- * computed again, a piece of the vocabulary at a time.  With bfloat16 operands
- * G is rounded to bfloat16; with float32 everything keeps float32's accuracy.
+ * computed again, a piece of the vocabulary at a time, and G of a piece is
+ * kept in the workspace (up to 4 GiB with the copies of the operands).
+ * With bfloat16 operands G is rounded to bfloat16.  With float32 the factors of
+ * both products are two float16 parts: G / dloss is kept to 2^-23 of itself and
+ * 2^-50, an element x of weight, and of dloss times hidden, to 2^-23 |x| +
+ * 2^-50 m with m the largest element of the WHOLE matrix.  So probabilities
+ * below 2^-27, features and rows 2^-27 of the largest and less lose relative
+ * accuracy, and what is below 2^-50 counts as zero; errors are small against
+ * the largest terms, not against every term.
  * dhidden and dweight must not overlap each other or an input.  lse has to be
  * the forward call's for the same operands: far smaller values take G beyond
  * the range it is kept in.

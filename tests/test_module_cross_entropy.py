@@ -456,3 +456,66 @@ def test_nothing_is_written_behind_the_workspace(config, dtype, tile, piece, N, 
         else:
             m.run([h, w, y, lse, dl])
         assert bool((m._space[need:] == 0x5a).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [0, 1])
+@pytest.mark.parametrize("N,V,D", [(200, 300, 64), (37, 2001, 90), (1500, 41, 33)])
+def test_float32_of_very_different_sizes(config, native, N, V, D):
+    """The bound that the header states, where it is reached: features and row weights over ten decades, probabilities
+    down to 1e-20.  An element x of a row or matrix whose largest is m is kept to 2^-23 |x| + 2^-50 m (two float16 parts
+    with the largest at 2^14 or above: the second part is off by half of 2^-24 there, 2^-11 smaller), G / dloss to
+    2^-23 of itself and 2^-50; products of two second parts, at most 2^-22, are within what _sums allows.
+
+    Sums: a matrix instruction aligns eight products at a time by the sum of their factors' exponents and cuts each at 2^-24
+    of the largest, where a factor below float16's normal numbers counts as the smallest of them, 2^-14, which is 2^-28
+    of the largest element at 2^14: 16384 * 2^-23 with 7.476e-4 * 0.01299 beside it loses 5.86e-8 = 0.98 * 2^-24 *
+    (2^14 * 2^-14), with 2^-5 * 2^-4 in place of the first 2^-33.  So the sums' error is that of the factors' sizes
+    raised to at least 2^-28 of the largest, 8 * 2^-24 of each group's largest product and so of the whole sum of sizes,
+    beside _sums for the accumulations."""
+    config("ce.native", native)
+    h, w, y, dl = _operands("float32", N, V, D, N + D, spread=40.0)
+    h *= 10.0 ** -(torch.arange(D, device="cuda") % 11)
+    w *= 10.0 ** (torch.arange(D, device="cuda") % 11 / 2)
+    dl *= 10.0 ** -(torch.arange(N, device="cuda") % 9)
+    h[1, :], w[1, :] = h[1, :] * 1e-6, w[1, :] * 1e-6
+    loss, lse, dh, dw = _run(h, w, y, dl, "float32")
+    H, W, dl = h.double(), w.double(), dl.double()
+    ok = (y >= 0) & (y < V)
+    n, at = torch.arange(N, device="cuda")[ok], y[ok].long()
+    kept, floor = 2.0 ** -23, 2.0 ** -50
+
+    def largest(x):
+        return x.abs().amax(1, keepdim=True)
+
+    def raised(x, most):
+        return torch.maximum(x.abs(), 2.0 ** -28 * most)
+
+    def sums(K):
+        return _sums(K, "float32") + 8 * 2.0 ** -24
+
+    logits = H @ W.T
+    d = sums(D) * (raised(H, largest(H)) @ raised(W, largest(W)).T)
+    d += floor * (largest(H) * W.abs().sum(1) + H.abs().sum(1)[:, None] * largest(W).T)
+    want = torch.logsumexp(logits, 1)
+    far = (logits - want[:, None]).abs().amax(1)
+    d_lse = d.amax(1) + (far * 2.0 ** -23 + 2.0 ** -21) + _sums(V, "bfloat16") + 2.0 ** -23 * want.abs()
+    assert bool(((lse.double() - want).abs() <= d_lse).all())
+    want_loss = torch.zeros_like(want)
+    want_loss[ok] = want[ok] - logits[n, at]
+    assert bool(((loss.double() - want_loss).abs() <= d_lse + d.amax(1) + 2.0 ** -23 * want_loss.abs()).all())
+    p = torch.exp(logits - want[:, None])
+    e = p * (d + (d_lse + far * 2.0 ** -23 + 2.0 ** -21)[:, None]) + 2.0 ** -22 * p
+    e[n, at] += 2.0 ** -22
+    P = p.clone()
+    P[n, at] -= 1.0
+    e += kept * P.abs() + floor
+    P[~ok], e[~ok] = 0.0, 0.0
+    F = torch.where(ok, dl, 0.0)[:, None] * H
+    assert float(p[ok].min()) < 2.0 ** -50 and float(F[ok].abs().max() / F[ok].abs().amin()) > 2.0 ** 30
+    for got, a, ea, b, K, f in ((dw, P.T, e.T, F, N, torch.ones(V, 1, device="cuda")), (dh, P, e, W, V, torch.where(ok, dl, 0.0)[:, None])):
+        eb = 1.5 * kept * b.abs() + floor * b.abs().max()      # a product with dloss is rounded as well
+        exact = f * (a @ b)
+        rounding = sums(K) * (raised(a, torch.ones_like(a)) @ raised(b, b.abs().max()))
+        tol = f * (ea @ (b.abs() + eb) + a.abs() @ eb + rounding) + 2 * HALF_STEP["float32"] * exact.abs() + TINY
+        assert bool(((got.double() - exact).abs() <= tol).all())
