@@ -576,21 +576,26 @@ template <typename T, typename Id>
 int lookup_typed(const void *table, const void *ids, void *out, int64_t n, int64_t V, int64_t D, float scale,
                  hipStream_t stream) {
   const T *t = static_cast<const T *>(table);
-  const Id *i = static_cast<const Id *>(ids);
-  T *o = static_cast<T *>(out);
   const int vec = vector_elements(D, sizeof(T), {table, out}), lpr = lanes_per_row(D, vec);
-  const dim3 grid(blocks_for((n + 3) / 4, lpr),
-                  static_cast<unsigned>(std::min<int64_t>(16, (D + lpr * vec - 1) / (lpr * vec))));
+  // A launch has fewer than 2^32 threads along x, and a row takes up to 16: 2^26 ids (2^30 threads) at a time.
+  constexpr int64_t kMostIds = 1 << 26;
+  for (int64_t from = 0; from < n; from += kMostIds) {
+    const Id *i = static_cast<const Id *>(ids) + from;
+    T *o = static_cast<T *>(out) + from * D;
+    const int64_t count = std::min(kMostIds, n - from);
+    const dim3 grid(blocks_for((count + 3) / 4, lpr),
+                    static_cast<unsigned>(std::min<int64_t>(16, (D + lpr * vec - 1) / (lpr * vec))));
 #define FG_LOOKUP(VEC)                                                                                          \
-  lookup_kernel<T, Id, VEC><<<grid, dim3(kBlockThreads), 0, stream>>>(t, i, o, n, static_cast<int32_t>(V),      \
+  lookup_kernel<T, Id, VEC><<<grid, dim3(kBlockThreads), 0, stream>>>(t, i, o, count, static_cast<int32_t>(V),  \
                                                                       static_cast<int32_t>(D), lpr, scale)
-  if constexpr (sizeof(T) == 2) {
-    if (vec == 8) FG_LOOKUP(8);
-  }
-  if (vec == 4) FG_LOOKUP(4);
-  if (vec == 2) FG_LOOKUP(2);
-  if (vec == 1) FG_LOOKUP(1);
+    if constexpr (sizeof(T) == 2) {
+      if (vec == 8) FG_LOOKUP(8);
+    }
+    if (vec == 4) FG_LOOKUP(4);
+    if (vec == 2) FG_LOOKUP(2);
+    if (vec == 1) FG_LOOKUP(1);
 #undef FG_LOOKUP
+  }
   FG_HIP_TRY(hipGetLastError());
   return FG_OK;
 }

@@ -300,3 +300,22 @@ def test_gradient_around_the_border_of_the_two_sorts(n, V, index):
     want = np.zeros((V, 3), np.float64)
     np.add.at(want, ids[ids >= 0], dout[ids >= 0])
     assert np.array_equal(got, want.astype(np.float32))
+
+
+@pytest.mark.gpu
+def test_more_ids_than_one_launch_has_threads_for():
+    """2^28 rows of 33 float16 take 16 threads each, 2^32 together, which is more than a launch may have."""
+    n, V, D = 2 ** 28 + 5, 7, 33
+    ids = torch.arange(n, dtype=torch.int32, device="cuda") % 9 - 1            # -1, 0 .. 6 and 7: padding on both sides
+    table = _normal((V, D), "float16", 1)
+    m = EmbeddingLookuphip(0.5)
+    m.build([placeholder((V, D), "float16"), placeholder((n,), "int32")])
+    m.out_tvm.tensor.fill_(float("nan"))
+    out = m.run([table, ids]).tensor
+    rows = torch.zeros(V + 2, D, dtype=torch.float16, device="cuda")
+    rows[1:V + 1] = table * 0.5                                                 # exact: no value is below 2^-13
+    assert float(table.abs().min()) >= 2.0 ** -13
+    step = 9 << 20
+    want = rows.repeat(step // 9, 1)
+    for at in range(0, n, step):
+        assert torch.equal(out[at:at + step], want[:min(step, n - at)])
