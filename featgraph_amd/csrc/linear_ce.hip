@@ -1,4 +1,4 @@
-// Softmax cross entropy of a linear scorer, without keeping the logits:
+// Softmax cross entropy of a linear scorer, without keeping the logits, and its gradients:
 //
 //   l[n, v]  = <h[n], w[v]>                    lse[n] = log sum over v of exp l[n, v]
 //   loss[n]  = lse[n] - l[n, y[n]]             (0 where the label y[n] is outside [0, V): the row is ignored)
@@ -13,12 +13,13 @@
 // elements of traffic against 6 N V D flops), bfloat16 rows that have to be padded in the same pass (19 rows x 137,737 classes
 // x 89: 103 -> 76 us); the copy of h also holds zeros in place of the rows to ignore.
 //
-// Where it stands (bfloat16), whole calls: 4096 rows x 65,536 classes x 1024: loss 450 us (1222 TFLOP/s), gradient 1512 (its
-// three products: 1091); a library's product of 8192^3 reaches 1333.  1024 x 232,965 x 128: 88 and 446, bound by the
+// Where it stands (bfloat16), whole calls: 4096 rows x 65,536 classes x 1024: loss 446 us (1233 TFLOP/s), gradient 1495 (its
+// three products: 1103); a library's product of 8192^3 reaches 1333.  1024 x 232,965 x 128: 89 to 100 and 447, bound by the
 // epilogues: an exponential per logit, P written once and read twice.
 //
-// Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step of each
-// term, random in sign; the results are rounded to bfloat16 themselves); everything between is float32.  float32
+// Types: bfloat16 operands are used as they are; P is stored times dloss, rounded to bfloat16 (half a step, 2^-8, of each
+// term: the matrix instructions take no wider type, two parts would double both products, and the results are rounded to
+// bfloat16 themselves); everything between is float32.  float32
 // operands, P among them, are split into two float16 parts (mfma_gemm.hpp); the loss multiplies them as they are where
 // reading one of them bounds it (few rows, or few classes).  P is at most 1 and stored times 2^14; dloss is applied to the
 // rows of dh in the epilogue and to the copy of h for dw.  What the parts keep: x of a row (logits) or of a whole matrix

@@ -84,7 +84,7 @@ struct MultiplyNative {
 struct GemmOperand {
   const uint16_t *p = nullptr;  // part 0
   int64_t part = 0;             // elements from one part to the next
-  int64_t row = kStepK;         // elements from one row to the next, a multiple of 8
+  int64_t row = kStepK;         // elements from one row to the next: a multiple of 8, native float32 of 2
   int64_t step = 0;             // elements from one step of k to the next
   int32_t rows = 0;
 };
