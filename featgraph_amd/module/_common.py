@@ -123,7 +123,10 @@ def check_apart(written, read, what):
 
 
 class DenseBase:
-    """What the modules without an adjacency matrix share: the device, run() over checked operands, timing."""
+    """What the modules without an adjacency matrix share: the device, run() over checked operands, timing.
+
+    build() allocates and enqueues nothing: a run writes every element of the arrays that its module owns, and a fill
+    left on the stream of build() could write into the results of a run on another stream."""
 
     _target = "hip"
 

@@ -58,7 +58,7 @@ class LinearCrossEntropyhip(_LinearCrossEntropyBase):
     def build(self, input_placeholders, compute_args=None, schedule_args=None):
         self._parse(input_placeholders, compute_args, schedule_args)
         self._space = self._workspace("fg_linear_ce_workspace", *self._sizes, self._element[1])
-        self._loss, self._lse = (NDArray(torch.zeros(self._label_shape, dtype=torch.float32, device=self._ctx)) for _ in range(2))
+        self._loss, self._lse = (NDArray(torch.empty(self._label_shape, dtype=torch.float32, device=self._ctx)) for _ in range(2))
         self.out_tvm = self._loss
         self._built = True
 
@@ -87,8 +87,8 @@ class LinearCrossEntropyGradhip(_LinearCrossEntropyBase):
     def build(self, input_placeholders, compute_args=None, schedule_args=None):
         self._parse(input_placeholders, compute_args, schedule_args)
         self._space = self._workspace("fg_linear_ce_grad_workspace", *self._sizes, self._element[1])
-        self._dhidden = NDArray(torch.zeros(self._hidden_shape, dtype=self._element[0], device=self._ctx))
-        self._dweight = NDArray(torch.zeros(self._weight_shape, dtype=self._element[0], device=self._ctx))
+        self._dhidden = NDArray(torch.empty(self._hidden_shape, dtype=self._element[0], device=self._ctx))
+        self._dweight = NDArray(torch.empty(self._weight_shape, dtype=self._element[0], device=self._ctx))
         self.out_tvm = self._dhidden
         self._built = True
 

@@ -50,7 +50,7 @@ class EmbeddingLookuphip(C.DenseBase):
         C.check_known_keys(compute_args, (), "compute_args")
         C.check_known_keys(schedule_args, (), "schedule_args")
         self._element, self._index, self._shape, self._ids_shape, self._n = _parse(input_placeholders)
-        self.out_tvm = NDArray(torch.zeros(self._ids_shape + self._shape[1:], dtype=self._element[0], device=self._ctx))
+        self.out_tvm = NDArray(torch.empty(self._ids_shape + self._shape[1:], dtype=self._element[0], device=self._ctx))
         self._built = True
 
     def _checked(self, arrays):
@@ -93,7 +93,7 @@ class EmbeddingLookupGradhip(C.DenseBase):
 
     def _own(self):
         if self.out_tvm is None:
-            self.out_tvm = NDArray(torch.zeros(self._shape, dtype=self._element[0], device=self._ctx))
+            self.out_tvm = NDArray(torch.empty(self._shape, dtype=self._element[0], device=self._ctx))
         return self.out_tvm
 
     def _checked(self, arrays):

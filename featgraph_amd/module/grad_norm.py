@@ -42,7 +42,7 @@ class GradNormhip(C.DenseBase):
 
     def _allocate(self):
         self._space = self._workspace("fg_grad_norm_workspace")
-        self._norm = NDArray(torch.zeros((), dtype=torch.float32, device=self._ctx))
+        self._norm = NDArray(torch.empty((), dtype=torch.float32, device=self._ctx))
         self.out_tvm = self._norm
 
     def _checked(self, arrays):
@@ -86,7 +86,7 @@ class ClipGradNormhip(GradNormhip):
         self._allocate()
         self._clipped = None
         if not self._in_place:
-            self._clipped = [NDArray(torch.zeros(shape, dtype=t, device=self._ctx)) for shape, t, _ in self._expected]
+            self._clipped = [NDArray(torch.empty(shape, dtype=t, device=self._ctx)) for shape, t, _ in self._expected]
             self._out[:] = [c.tensor.data_ptr() for c in self._clipped]
             spans = sorted([(c.tensor.data_ptr(), size) for c, (_, _, size) in zip(self._clipped, self._expected) if size] +
                            [(self._norm.tensor.data_ptr(), 4)])

@@ -169,3 +169,43 @@ def test_two_runs_on_two_streams():
 
 def test_config_keys_of_the_products():
     assert _lib.config_get("ce.tile") == 0 and _lib.config_get("ce.piece_rows") == 0
+
+
+def test_build_leaves_nothing_to_do_on_its_stream():
+    """Modules built while their stream is busy, and run at once on another one: nothing that build() enqueued may
+    arrive later and write into the results."""
+    V, n, D = 300, 70, 40
+    g = torch.Generator().manual_seed(5)
+    table, dout = torch.randn(V, D, generator=g).cuda(), torch.randn(n, D, generator=g).cuda()
+    ids = torch.randint(0, V, (n,), generator=g).cuda()
+    hidden, dloss = torch.randn(n, D, generator=g).cuda(), torch.rand(n, generator=g).cuda() + 0.5
+    ph = [placeholder((V, D)), placeholder((n,), "int64")]
+    triple = [placeholder((n, D))] + ph
+
+    def build():
+        m = (EmbeddingLookuphip(2.0), EmbeddingLookupGradhip(2.0), LinearCrossEntropyhip(), LinearCrossEntropyGradhip(), ClipGradNormhip(0.5))
+        for x, p in zip(m, (ph, ph, triple, triple, [placeholder((V, D)), placeholder((n, D))])):
+            x.build(p)
+        return m
+
+    def run(m):
+        rows, grad = m[0].run([table, ids]), m[1].run([ids, dout])
+        loss, lse = m[2].run([hidden, table, ids])
+        dh, dw = m[3].run([hidden, table, ids, lse, dloss])
+        norm, clipped = m[4].run([table, dout])
+        return [x.tensor for x in (rows, grad, loss, lse, dh, dw, norm, *clipped)]
+
+    first = build()
+    want = [x.clone() for x in run(first)]
+    a = torch.randn(8192, 8192, device="cuda")
+    b = torch.empty_like(a)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(6):                      # some 40 ms of work
+        torch.mm(a, a, out=b)
+    m = build()
+    with torch.cuda.stream(side):
+        got = run(m)
+    side.synchronize()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
